@@ -51,6 +51,40 @@ class MoeTrace(C.Structure):
                                   "moe_shared", "moe_out")]
 
 
+class KvCache(C.Structure):
+    """ApusCudaKvCache: device addresses (ints) and sizes"""
+    _fields_ = [(k, vp) for k in ("k", "v", "refs", "table", "len", "work")] + \
+        [(k, sz) for k in ("layers", "pages", "page_tokens", "kv_heads", "head_dim", "seqs",
+                           "max_pages")]
+
+
+def kv_work_ints(pages, seqs):
+    """APUS_CUDA_KV_WORK_INTS"""
+    return 4 * pages + 4 * seqs + 64
+
+
+class Rope(C.Structure):
+    """ApusCudaRope"""
+    _fields_ = [(k, vp) for k in ("q", "k", "v", "q_out", "k_out")] + \
+        [(k, sz) for k in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride",
+                           "rows", "heads", "kv_heads", "head_dim", "rot_dim")] + \
+        [("pos", vp), ("axes", sz), ("sections", sz * 4), ("interleaved", C.c_int),
+         ("theta", C.c_double)]
+
+
+class Attn(C.Structure):
+    """ApusCudaAttn"""
+    _fields_ = [(k, vp) for k in ("q", "gate", "out", "lse")] + \
+        [(k, sz) for k in ("q_stride", "gate_stride", "out_stride", "rows", "heads", "kv_heads",
+                           "head_dim")] + [("scale", C.c_float)]
+
+
+class AttnKeys(C.Structure):
+    """ApusCudaAttnKeys"""
+    _fields_ = [(k, vp) for k in ("k", "v", "cu_q", "cu_k")] + \
+        [(k, sz) for k in ("k_stride", "v_stride", "rows", "seqs")] + [("causal", C.c_int)]
+
+
 # every symbol include/backend_cuda.h declares
 SYMBOLS = [
     "apus_cuda_enable", "apus_cuda_disable", "apus_cuda_is_enabled",
@@ -82,7 +116,10 @@ SYMBOLS = [
     "apus_cuda_ep_pull_experts_dev",
     "apus_cuda_route_dev", "apus_cuda_dispatch_dev",
     "apus_cuda_dispatch_dev_static", "apus_cuda_rmsnorm_dev",
-    "apus_cuda_resadd_dev", "apus_cuda_bf16_gemv_dev", "apus_synth_fill_host",
+    "apus_cuda_resadd_dev", "apus_cuda_bf16_gemv_dev", "apus_cuda_kv_extend_dev",
+    "apus_cuda_kv_fork_dev", "apus_cuda_kv_free_dev", "apus_cuda_kv_compact_dev",
+    "apus_cuda_kv_copy_dev", "apus_cuda_rope_dev", "apus_cuda_attn_prompt_dev",
+    "apus_cuda_attn_decode_dev", "apus_synth_fill_host",
     "apus_synth_fill_dev",
 ]
 
@@ -177,6 +214,15 @@ class Backend:
         L.apus_cuda_rmsnorm_dev.argtypes = [vp, vp, vp, sz, sz, vp]
         L.apus_cuda_resadd_dev.argtypes = [vp, vp, vp, sz, vp]
         L.apus_cuda_bf16_gemv_dev.argtypes = [vp, vp, vp, sz, sz, sz, vp]
+        kv = C.POINTER(KvCache)
+        L.apus_cuda_kv_extend_dev.argtypes = [kv, vp, vp, sz, vp, sz, vp]
+        L.apus_cuda_kv_fork_dev.argtypes = [kv, vp, vp, sz, vp]
+        L.apus_cuda_kv_free_dev.argtypes = [kv, vp, sz, vp]
+        L.apus_cuda_kv_compact_dev.argtypes = [kv, vp]
+        L.apus_cuda_kv_copy_dev.argtypes = [kv, vp, vp, sz, vp]
+        L.apus_cuda_rope_dev.argtypes = [C.POINTER(Rope), kv, sz, vp, vp]
+        L.apus_cuda_attn_prompt_dev.argtypes = [C.POINTER(Attn), C.POINTER(AttnKeys), vp]
+        L.apus_cuda_attn_decode_dev.argtypes = [C.POINTER(Attn), kv, sz, vp, vp]
         L.apus_synth_fill_host.argtypes = [u16p, sz, C.c_uint64, C.c_uint32,
                                            C.c_uint32, C.c_uint64, C.c_double]
         L.apus_synth_fill_host.restype = None
@@ -604,6 +650,39 @@ class Backend:
     def bf16_gemv_dev(self, d_w, d_x, d_y, M, O, K, stream=None):
         self._check(self.lib.apus_cuda_bf16_gemv_dev(d_w, d_x, d_y, M, O, K, stream),
                     "apus_cuda_bf16_gemv_dev")
+
+    # ---- the attention half (structs of device addresses) -----------------------
+    def kv_extend_dev(self, kv, d_seq, d_cu, n, d_slot=None, rows=0, stream=None):
+        self._check(self.lib.apus_cuda_kv_extend_dev(C.byref(kv), d_seq, d_cu, n, d_slot, rows,
+                                                     stream), "apus_cuda_kv_extend_dev")
+
+    def kv_fork_dev(self, kv, d_src, d_dst, n, stream=None):
+        self._check(self.lib.apus_cuda_kv_fork_dev(C.byref(kv), d_src, d_dst, n, stream),
+                    "apus_cuda_kv_fork_dev")
+
+    def kv_free_dev(self, kv, d_seq, n, stream=None):
+        self._check(self.lib.apus_cuda_kv_free_dev(C.byref(kv), d_seq, n, stream),
+                    "apus_cuda_kv_free_dev")
+
+    def kv_compact_dev(self, kv, stream=None):
+        self._check(self.lib.apus_cuda_kv_compact_dev(C.byref(kv), stream),
+                    "apus_cuda_kv_compact_dev")
+
+    def kv_copy_dev(self, kv, d_src, d_dst, n, stream=None):
+        self._check(self.lib.apus_cuda_kv_copy_dev(C.byref(kv), d_src, d_dst, n, stream),
+                    "apus_cuda_kv_copy_dev")
+
+    def rope_dev(self, rope, kv=None, layer=0, d_slot=None, stream=None):
+        self._check(self.lib.apus_cuda_rope_dev(C.byref(rope), C.byref(kv) if kv else None, layer,
+                                                d_slot, stream), "apus_cuda_rope_dev")
+
+    def attn_prompt_dev(self, attn, keys, stream=None):
+        self._check(self.lib.apus_cuda_attn_prompt_dev(C.byref(attn), C.byref(keys), stream),
+                    "apus_cuda_attn_prompt_dev")
+
+    def attn_decode_dev(self, attn, kv, layer, d_seq=None, stream=None):
+        self._check(self.lib.apus_cuda_attn_decode_dev(C.byref(attn), C.byref(kv), layer, d_seq,
+                                                       stream), "apus_cuda_attn_decode_dev")
 
     # ---- synthetic tensors -------------------------------------------------------
     def synth_fill_host(self, n, seed, layer, tensor_id, sigma, first=0):

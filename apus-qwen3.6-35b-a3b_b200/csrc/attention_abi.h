@@ -1,0 +1,350 @@
+/*
+ * attention_abi.h — C-ABI of the attention half's operators (include/backend_cuda.h): checks
+ * of arguments, views for the kernels, launches.  Part of backend_cuda.cu, which holds the
+ * context, the order of calls on different streams and the error text.
+ */
+#pragma once
+
+/* calls run on the backend's device whatever the thread's current one is */
+struct DeviceGuard {
+    int old = -1;
+    bool changed = false;
+    explicit DeviceGuard(int device) {
+        if (cudaGetDevice(&old) == cudaSuccess && old != device)
+            changed = cudaSetDevice(device) == cudaSuccess;
+    }
+    ~DeviceGuard() {
+        if (changed) cudaSetDevice(old);
+    }
+};
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int kv_view(const ApusCudaKvCache *kv, const char *what, KvView *out) {
+    if (!kv || !kv->k || !kv->v || !kv->refs || !kv->table || !kv->len || !kv->work)
+        return fail("%s: the cache has a null pointer", what);
+    if (!kv->layers || !kv->pages || !kv->kv_heads || !kv->seqs || !kv->max_pages)
+        return fail("%s: the cache has a zero size", what);
+    if (!kv->page_tokens || kv->page_tokens % 16 || kv->page_tokens > 256)
+        return fail("%s: page_tokens must be a multiple of 16, at most 256", what);
+    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+        return fail("%s: head_dim must be 64, 128 or 256", what);
+    if (!aligned16(kv->k) || !aligned16(kv->v))
+        return fail("%s: the pools must be 16-byte aligned", what);
+    const size_t most = 0x7fffffff;
+    if (kv->pages > most / kv->page_tokens || kv->max_pages > most / kv->page_tokens ||
+        kv->layers > 65536 || kv->kv_heads > 1024 || kv->seqs > most / 64 ||
+        kv->kv_heads * kv->page_tokens > most / kv->head_dim)
+        return fail("%s: the cache is too large", what);
+    KvView v;
+    v.k = kv->k;
+    v.v = kv->v;
+    v.refs = kv->refs;
+    v.table = kv->table;
+    v.len = kv->len;
+    v.work = kv->work;
+    v.layers = (int)kv->layers;
+    v.pages = (int)kv->pages;
+    v.page_tokens = (int)kv->page_tokens;
+    v.seqs = (int)kv->seqs;
+    v.max_pages = (int)kv->max_pages;
+    v.page_elems = (int)(kv->kv_heads * kv->page_tokens * kv->head_dim);
+    *out = v;
+    return 0;
+}
+
+#define LAUNCH_OK(call)                                                          \
+    do {                                                                         \
+        cudaError_t e_ = (call);                                                 \
+        if (e_ != cudaSuccess) {                                                 \
+            cudaGetLastError();                                                  \
+            return fail("kernel launch: %s (%s:%d)", cudaGetErrorString(e_),     \
+                        __FILE__, __LINE__);                                     \
+        }                                                                        \
+        g_ctx->launches++;                                                       \
+    } while (0)
+
+static unsigned kv_apply_grid(const Ctx *c) {
+    return (unsigned)c->sm_count * (2048 / KV_APPLY_THREADS);
+}
+
+extern "C" int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t *d_seq,
+                                       const int32_t *d_cu, size_t n, int32_t *d_slot,
+                                       size_t rows, void *stream) {
+    KvView v;
+    if (kv_view(kv, "kv_extend_dev", &v)) return 1;
+    if (!n) return 0;
+    if (!d_cu || n > kv->seqs || (d_slot && rows > 0x7fffffff))
+        return fail("kv_extend_dev: bad args");
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    LAUNCH_OK(launch_k(kv_extend_kernel, dim3(1), dim3(KV_PLAN_THREADS), 0, (cudaStream_t)stream,
+                       v, d_seq, d_cu, (int)n, d_slot, (int)rows));
+    return 0;
+}
+
+extern "C" int apus_cuda_kv_free_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, size_t n,
+                                     void *stream) {
+    KvView v;
+    if (kv_view(kv, "kv_free_dev", &v)) return 1;
+    if (!n) return 0;
+    if (n > 0x7fffffff || (!d_seq && n > kv->seqs)) return fail("kv_free_dev: bad args");
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    const size_t most = (size_t)g_ctx->sm_count * 16;
+    LAUNCH_OK(launch_k(kv_free_kernel, dim3((unsigned)(n < most ? n : most)), dim3(128), 0,
+                       (cudaStream_t)stream, v, d_seq, (int)n));
+    return 0;
+}
+
+extern "C" int apus_cuda_kv_fork_dev(const ApusCudaKvCache *kv, const int32_t *d_src,
+                                     const int32_t *d_dst, size_t n, void *stream) {
+    KvView v;
+    if (kv_view(kv, "kv_fork_dev", &v)) return 1;
+    if (!n) return 0;
+    if (!d_src || !d_dst || n > kv->seqs) return fail("kv_fork_dev: bad args");
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    LAUNCH_OK(launch_k(kv_fork_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS), 0, st, v, d_src,
+                       d_dst, (int)n));
+    LAUNCH_OK(launch_k(kv_apply_kernel<KV_APPLY_FORK>, dim3(kv_apply_grid(g_ctx)),
+                       dim3(KV_APPLY_THREADS), 0, st, v, d_src, d_dst, (int)n));
+    return 0;
+}
+
+extern "C" int apus_cuda_kv_compact_dev(const ApusCudaKvCache *kv, void *stream) {
+    KvView v;
+    if (kv_view(kv, "kv_compact_dev", &v)) return 1;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int32_t *none = nullptr;
+    LAUNCH_OK(launch_k(kv_compact_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS), 0, st, v));
+    LAUNCH_OK(launch_k(kv_apply_kernel<KV_APPLY_COMPACT>, dim3(kv_apply_grid(g_ctx)),
+                       dim3(KV_APPLY_THREADS), 0, st, v, none, none, 0));
+    return 0;
+}
+
+extern "C" int apus_cuda_kv_copy_dev(const ApusCudaKvCache *kv, const int32_t *d_src,
+                                     const int32_t *d_dst, size_t n, void *stream) {
+    KvView v;
+    if (kv_view(kv, "kv_copy_dev", &v)) return 1;
+    if (!n) return 0;
+    if (!d_src || !d_dst || n > kv->pages) return fail("kv_copy_dev: bad args");
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    LAUNCH_OK(launch_k(kv_copy_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS), 0, st, v, d_src,
+                       d_dst, (int)n));
+    LAUNCH_OK(launch_k(kv_apply_kernel<KV_APPLY_COPY>, dim3(kv_apply_grid(g_ctx)),
+                       dim3(KV_APPLY_THREADS), 0, st, v, d_src, d_dst, (int)n));
+    return 0;
+}
+
+/* a tensor of rows: its stride, or 0 where it is none that the kernels can read */
+static long row_stride(const void *p, size_t stride, size_t heads, size_t head_dim) {
+    const size_t s = stride ? stride : heads * head_dim;
+    if (!p || !aligned16(p) || s % 8 || s < heads * head_dim || s > ((size_t)1 << 40)) return 0;
+    return (long)s;
+}
+
+static int heads_check(const char *what, size_t heads, size_t kv_heads, size_t head_dim) {
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail("%s: head_dim must be 64, 128 or 256", what);
+    if (!heads || !kv_heads || heads % kv_heads || heads / kv_heads > 16 || kv_heads > 1024)
+        return fail("%s: heads must be a multiple of kv_heads, at most 16 times as many", what);
+    return 0;
+}
+
+extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *kv, size_t layer,
+                                  const int32_t *d_slot, void *stream) {
+    if (!r) return fail("rope_dev: bad args");
+    if (heads_check("rope_dev", r->heads, r->kv_heads, r->head_dim)) return 1;
+    if (!r->rot_dim || r->rot_dim % 16 || r->rot_dim > r->head_dim)
+        return fail("rope_dev: rot_dim must be a multiple of 16, at most head_dim");
+    if (!r->axes || r->axes > 4 || !(r->theta > 0.0) || r->theta > 1e30)
+        return fail("rope_dev: 1 to 4 axes and a positive theta");
+    RopeParams p = {};
+    const size_t pairs = r->rot_dim / 2;
+    size_t count[4] = {}, sum = 0;
+    for (size_t a = 0; a < r->axes; a++) {
+        if (r->sections[a] > pairs) return fail("rope_dev: sections must add up to rot_dim / 2");
+        sum += r->sections[a];
+    }
+    if (sum != pairs) return fail("rope_dev: sections must add up to rot_dim / 2");
+    for (size_t i = 0, a = 0, in = 0; i < pairs; i++) {
+        if (r->interleaved) {
+            a = i % r->axes;
+            if (count[a] >= r->sections[a]) a = 0;
+        } else {
+            while (in >= r->sections[a]) {
+                a++;
+                in = 0;
+            }
+            in++;
+        }
+        count[a]++;
+        p.axis[i] = (unsigned char)a;
+        p.turns[i] = pow(r->theta, -2.0 * (double)i / (double)r->rot_dim) /
+                     6.283185307179586476925286766559;
+    }
+    for (size_t a = 0; a < r->axes; a++)
+        if (count[a] != r->sections[a])
+            return fail("rope_dev: the sections cannot be interleaved over these axes");
+    KvView v = {};
+    if (kv) {
+        if (kv_view(kv, "rope_dev", &v)) return 1;
+        if (kv->kv_heads != r->kv_heads || kv->head_dim != r->head_dim || layer >= kv->layers)
+            return fail("rope_dev: the cache has other heads or fewer layers");
+    }
+    if (!r->rows) return 0;
+    if (r->rows > (1u << 30) || !r->pos || (kv && !d_slot)) return fail("rope_dev: bad args");
+    p.q_stride = row_stride(r->q, r->q_stride, r->heads, r->head_dim);
+    p.k_stride = row_stride(r->k, r->k_stride, r->kv_heads, r->head_dim);
+    p.q_out_stride = row_stride(r->q_out, r->q_out_stride, r->heads, r->head_dim);
+    p.k_out_stride = r->k_out ? row_stride(r->k_out, r->k_out_stride, r->kv_heads, r->head_dim) : 1;
+    p.v_stride = kv ? row_stride(r->v, r->v_stride, r->kv_heads, r->head_dim) : 1;
+    if (!p.q_stride || !p.k_stride || !p.q_out_stride || !p.k_out_stride || !p.v_stride ||
+        (!kv && !r->k_out))
+        return fail("rope_dev: a tensor is missing, or its address or stride is not a multiple "
+                    "of 16 bytes or less than a row");
+    p.q = r->q;
+    p.k = r->k;
+    p.v = r->v;
+    p.q_out = r->q_out;
+    p.k_out = r->k_out;
+    p.rows = (int)r->rows;
+    p.heads = (int)r->heads;
+    p.kv_heads = (int)r->kv_heads;
+    p.head_dim = (int)r->head_dim;
+    p.rot = (int)r->rot_dim;
+    p.pos = r->pos;
+    if (kv) {
+        p.slot = d_slot;
+        const size_t at = layer * kv->pages * (size_t)v.page_elems;
+        p.cache_k = kv->k + at;
+        p.cache_v = kv->v + at;
+        p.page_tokens = v.page_tokens;
+        p.pages = v.pages;
+        p.status = kv->work;
+    }
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    /* tokens to a CTA: as many as give every thread an angle, fewer where that leaves SMs idle */
+    size_t tokens = ROPE_THREADS / pairs ? ROPE_THREADS / pairs : 1;
+    while (tokens > 1 && (r->rows + tokens - 1) / tokens < 2 * (size_t)g_ctx->sm_count)
+        tokens /= 2;
+    p.tokens = (int)tokens;
+    LAUNCH_OK(launch_k(rope_kernel, dim3((unsigned)((r->rows + tokens - 1) / tokens)),
+                       dim3(ROPE_THREADS), tokens * pairs * sizeof(float2), (cudaStream_t)stream,
+                       p));
+    return 0;
+}
+
+static int attn_view(const ApusCudaAttn *a, const char *what, AttnView *out) {
+    if (heads_check(what, a->heads, a->kv_heads, a->head_dim)) return 1;
+    if (!(a->scale > 0.0f) || a->scale > 1e30f) return fail("%s: scale must be positive", what);
+    if (a->rows > (1u << 30)) return fail("%s: too many rows", what);
+    AttnView v = {};
+    v.rows = (int)a->rows;
+    v.heads = (int)a->heads;
+    v.group = (int)(a->heads / a->kv_heads);
+    v.scale = a->scale;
+    *out = v;
+    if (!a->rows) return 0;
+    v.q = a->q;
+    v.gate = a->gate;
+    v.out = a->out;
+    v.lse = a->lse;
+    v.q_stride = row_stride(a->q, a->q_stride, a->heads, a->head_dim);
+    v.out_stride = row_stride(a->out, a->out_stride, a->heads, a->head_dim);
+    v.gate_stride = a->gate ? row_stride(a->gate, a->gate_stride, a->heads, a->head_dim) : 1;
+    if (!v.q_stride || !v.out_stride || !v.gate_stride)
+        return fail("%s: q, gate or out is missing, or its address or stride is not a multiple "
+                    "of 16 bytes or less than a row", what);
+    *out = v;
+    return 0;
+}
+
+template <bool PAGED>
+static int launch_rows(const AttnView &a, size_t D, const AttnPacked &pk, const AttnPaged &pg,
+                       cudaStream_t st) {
+    const dim3 grid((unsigned)(((size_t)a.rows * a.heads + 7) / 8));
+    if (D == 64) LAUNCH_OK(launch_k(attn_rows_kernel<64, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
+    else if (D == 128) LAUNCH_OK(launch_k(attn_rows_kernel<128, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
+    else LAUNCH_OK(launch_k(attn_rows_kernel<256, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
+    return 0;
+}
+
+extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *keys,
+                                         void *stream) {
+    if (!a || !keys) return fail("attn_prompt_dev: bad args");
+    AttnView v;
+    if (attn_view(a, "attn_prompt_dev", &v)) return 1;
+    if (keys->rows > (1u << 30) || keys->seqs > (1u << 24))
+        return fail("attn_prompt_dev: too many keys or sequences");
+    if (!a->rows || !keys->seqs) return 0;
+    if (!keys->cu_q || !keys->cu_k) return fail("attn_prompt_dev: bad args");
+    AttnPacked pk = {};
+    pk.k = keys->k;
+    pk.v = keys->v;
+    pk.cu_q = keys->cu_q;
+    pk.cu_k = keys->cu_k;
+    pk.rows = (int)keys->rows;
+    pk.seqs = (int)keys->seqs;
+    pk.causal = keys->causal != 0;
+    if (keys->rows) {
+        pk.k_stride = row_stride(keys->k, keys->k_stride, a->kv_heads, a->head_dim);
+        pk.v_stride = row_stride(keys->v, keys->v_stride, a->kv_heads, a->head_dim);
+        if (!pk.k_stride || !pk.v_stride)
+            return fail("attn_prompt_dev: k or v is missing, or its address or stride is not a "
+                        "multiple of 16 bytes or less than a row");
+    }
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    Ordered ord(g_ctx, st);
+    if (ord.rc) return 1;
+    return launch_rows<false>(v, a->head_dim, pk, AttnPaged{}, st);
+}
+
+extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv,
+                                         size_t layer, const int32_t *d_seq, void *stream) {
+    if (!a) return fail("attn_decode_dev: bad args");
+    AttnView v;
+    KvView c;
+    if (attn_view(a, "attn_decode_dev", &v)) return 1;
+    if (kv_view(kv, "attn_decode_dev", &c)) return 1;
+    if (kv->kv_heads != a->kv_heads || kv->head_dim != a->head_dim || layer >= kv->layers)
+        return fail("attn_decode_dev: the cache has other heads or fewer layers");
+    if (!d_seq && a->rows > kv->seqs) return fail("attn_decode_dev: more rows than sequences");
+    if (!a->rows) return 0;
+    AttnPaged pg = {};
+    const size_t at = layer * kv->pages * (size_t)c.page_elems;
+    pg.k = kv->k + at;
+    pg.v = kv->v + at;
+    pg.table = kv->table;
+    pg.len = kv->len;
+    pg.seq = d_seq;
+    pg.status = kv->work;
+    pg.pages = c.pages;
+    pg.page_tokens = c.page_tokens;
+    pg.seqs = c.seqs;
+    pg.max_pages = c.max_pages;
+    pg.kv_heads = (int)kv->kv_heads;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    Ordered ord(g_ctx, st);
+    if (ord.rc) return 1;
+    return launch_rows<true>(v, a->head_dim, AttnPacked{}, pg, st);
+}

@@ -13,6 +13,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -21,6 +22,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attn_rows.cuh"
 #include "common.cuh"
 #include "decode_fused.cuh"
 #include "decode_stack.cuh"
@@ -33,9 +35,11 @@
 #include "place.cuh"
 #include "exact_dense.cuh"
 #include "host_stage.h"
+#include "kv_pages.cuh"
 #include "misc_kernels.cuh"
 #include "prefill_gemm.cuh"
 #include "pair_gemm.cuh"
+#include "rope.cuh"
 #include "router.cuh"
 #include "slab_loader.h"
 
@@ -2978,6 +2982,12 @@ extern "C" int apus_cuda_resadd_dev(const uint16_t *d_a, const uint16_t *d_b,
     LAUNCHED();
     return 0;
 }
+
+/* ------------------------------------------------------------------------ */
+/* the attention half's operators                                            */
+/* ------------------------------------------------------------------------ */
+
+#include "attention_abi.h"
 
 /* ------------------------------------------------------------------------ */
 /* synthetic tensors                                                         */

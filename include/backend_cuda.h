@@ -550,6 +550,121 @@ int apus_cuda_resadd_dev(const uint16_t *d_a, const uint16_t *d_b,
 int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *d_y,
                             size_t M, size_t O, size_t K, void *stream);
 
+/* ---- the attention half's operators --------------------------------------
+ * Net-new beside the engine's CPU kernels (c/attn.h: one sequence, one plain cache): what a
+ * server needs between the projections of a full-attention layer.  All pointers are device
+ * pointers of the backend's device, BF16 tensors as codes; calls enqueue on `stream`, do not
+ * synchronise, allocate nothing once the backend is enabled, and may be captured in a graph.
+ * Tensors are addressed by rows: `stride` elements from one row (token) to the next (0: heads *
+ * head_dim), heads side by side within a row; addresses and strides in multiples of 16 bytes.
+ * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 times as many: head h
+ * reads key head h / (heads / kv_heads). */
+
+/* A cache of keys and values in pages, for the caller's own device memory (nothing is owned by
+ * the library).  A page holds page_tokens tokens (a multiple of 16, at most 256) of every head;
+ * page p of layer l and head h starts at element
+ *     ((l * pages + p) * kv_heads + h) * page_tokens * head_dim
+ * of k and of v.  Token t of sequence s is token t % page_tokens of page
+ * table[s * max_pages + t / page_tokens].  refs counts the sequences that hold a page, 0 is a
+ * free one.  A new cache has refs 0, len 0, table -1 and work 0 (k and v as they are).  Entries of the table behind a
+ * sequence's last page are not read.  pages * page_tokens < 2^31.
+ *
+ * work is scratch of the calls on this cache; its first word is the cache's status, which
+ * stays at the first thing that went wrong until the caller clears it: 0 ok, 1 pages ran
+ * out, 2 a list names what it must not, 3 a page number outside of the pool (or a page given
+ * back too often).  A kv_ call that cannot do all that its list asks for leaves everything as
+ * it was (kv_free: what the bad entries name). */
+typedef struct {
+    uint16_t *k, *v;       /* [layers][pages][kv_heads][page_tokens][head_dim] */
+    int32_t *refs;         /* [pages] */
+    int32_t *table;        /* [seqs][max_pages] */
+    int32_t *len;          /* [seqs] tokens held */
+    int32_t *work;         /* [APUS_CUDA_KV_WORK_INTS(pages, seqs)] */
+    size_t layers, pages, page_tokens, kv_heads, head_dim, seqs, max_pages;
+} ApusCudaKvCache;
+#define APUS_CUDA_KV_WORK_INTS(pages, seqs) (4 * (size_t)(pages) + 4 * (size_t)(seqs) + 64)
+
+/* Room for more tokens: sequence d_seq[i] (NULL: i) grows by d_cu[i+1] - d_cu[i] tokens, i < n,
+ * taking the lowest free pages in the order of the list; the tokens' keys and values are for
+ * the caller to write (apus_cuda_rope_dev).  d_slot [rows] (optional): the place of packed row t
+ * of d_cu, page * page_tokens + offset; -1 for rows outside of [d_cu[0], d_cu[n]) and for all
+ * rows where the call is refused (pages run out, a sequence twice in the list or longer than
+ * max_pages). */
+int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, const int32_t *d_cu,
+                            size_t n, int32_t *d_slot, size_t rows, void *stream);
+/* Sequences d_dst[i] (empty, none twice, none a source as well) become copies of d_src[i]: full
+ * pages are shared, a last page that is not full is copied in all layers, so that no page with
+ * two owners is ever written. */
+int apus_cuda_kv_fork_dev(const ApusCudaKvCache *kv, const int32_t *d_src, const int32_t *d_dst,
+                          size_t n, void *stream);
+/* Sequences d_seq[i] (NULL: i) end: their length is 0, their pages have one owner less, their entries of
+ * the table are -1. */
+int apus_cuda_kv_free_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, size_t n,
+                          void *stream);
+/* The pages in use move to the front of the pool: those at or behind the number of pages in
+ * use go, in ascending order, to the free ones before it. */
+int apus_cuda_kv_compact_dev(const ApusCudaKvCache *kv, void *stream);
+/* Contents of pages d_src[i] to pages d_dst[i] in all layers (no target twice, none a source as
+ * well).  Owners stay as they are. */
+int apus_cuda_kv_copy_dev(const ApusCudaKvCache *kv, const int32_t *d_src, const int32_t *d_dst,
+                          size_t n, void *stream);
+
+/* Rotary positions: pair i of a head, (x[i], x[i + rot_dim/2]), i < rot_dim/2, turns by
+ * pos[axis(i)] * theta^(-2 i / rot_dim); the rest of the head is passed on.  rot_dim a multiple
+ * of 16.  sections[a] pairs belong to axis a, one axis after the other, or, interleaved, pair i
+ * to axis i % axes as long as that axis has pairs left, else to axis 0.  q_out may be q and
+ * k_out k (same stride).  Angles are exact to 2^-23 of a turn for every int32 position. */
+typedef struct {
+    const uint16_t *q, *k, *v;        /* v: only for a cache */
+    uint16_t *q_out, *k_out;          /* k_out NULL: the cache alone gets the keys */
+    size_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    size_t rows, heads, kv_heads, head_dim, rot_dim;
+    const int32_t *pos;               /* [axes][rows] */
+    size_t axes, sections[4];
+    int interleaved;
+    double theta;
+} ApusCudaRope;
+/* With kv: the rotated keys and the values also go to place d_slot[row] of `layer` (negative:
+ * nowhere; see apus_cuda_kv_extend_dev; no place twice).  kv NULL: no cache, d_slot is not read. */
+int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *kv, size_t layer,
+                       const int32_t *d_slot, void *stream);
+
+/* What both forms of attention take: s_j = scale q . k_j over the keys that a row sees,
+ * p = softmax(s), out = (sum_j p_j v_j) * sigmoid(gate), narrowed once; lse = log sum_j exp(s_j).
+ * Sums and statistics are fp32; p is narrowed to BF16 for its product with v.  A row that sees no
+ * key gets zeros and -inf.  out overlaps no input. */
+typedef struct {
+    const uint16_t *q;                /* [rows][heads][head_dim] */
+    const uint16_t *gate;             /* the same, or NULL: no gate */
+    uint16_t *out;
+    float *lse;                       /* [rows][heads], or NULL */
+    size_t q_stride, gate_stride, out_stride;
+    size_t rows, heads, kv_heads, head_dim;
+    float scale;                      /* > 0 */
+} ApusCudaAttn;
+
+/* Attention of packed prompts: rows [cu_q[i], cu_q[i+1]) of q are the last ones of sequence i,
+ * whose keys and values are rows [cu_k[i], cu_k[i+1]) of k and v.  Causal: the last row sees all
+ * of them, each row before it one less; a sequence with more rows than keys has rows that see
+ * none.  Rows of out and lse outside of [cu_q[0], cu_q[seqs]) stay as they are.  No value of
+ * another sequence, or of a key behind the last one that a tile of rows may see, reaches a row,
+ * whatever it is.  (Among the tokens of one such tile, at most 128 rows of one key head, a
+ * value that is not finite spreads, as it does in a matrix product with zeros.) */
+typedef struct {
+    const uint16_t *k, *v;            /* [rows][kv_heads][head_dim] */
+    const int32_t *cu_q, *cu_k;       /* [seqs + 1] */
+    size_t k_stride, v_stride, rows, seqs;
+    int causal;
+} ApusCudaAttnKeys;
+int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *keys, void *stream);
+
+/* Attention of one new token a sequence over the paged cache: row b of q sees all
+ * len[d_seq[b]] tokens (d_seq NULL: len[b]) of `layer`, its own among them once written.  A row
+ * whose d_seq is negative stays as it is (a padded batch).  A page number outside of the pool
+ * leaves its tokens out and status 3 in the cache's work. */
+int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv, size_t layer,
+                              const int32_t *d_seq, void *stream);
+
 /* ---- synthetic tensors (benchmarks and tests) ---------------------------- */
 /* Fill n BF16 elements with the counter-based approximately-normal stream
  * (seed, layer, tensor_id), element index starting at first, scaled by

@@ -1,0 +1,310 @@
+"""Attention of packed prompts and of single tokens over the paged cache, against 64-bit
+softmax sums of the same inputs; rows that see nothing, padded batches, strides, values that
+are not finite where nothing may see them, streams and graphs."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(16, 2, 256), (32, 8, 128), (20, 4, 128), (12, 12, 64), (16, 1, 128), (6, 2, 64),
+         (3, 3, 256)]
+
+
+def _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, causal=True, gate=True, pad=0, seed=0,
+            scale=None, spoil=False):
+    import attn_util as u
+    import apus_b200.backend as B
+    rows, keys = sum(nq) + pad, sum(nk)
+    q, g = u.normal(rows, 2, heads, dim, seed=seed, scale=1.5).unbind(1)
+    k, v = u.normal(keys + 9, 2, kv_heads, dim, seed=seed + 1).unbind(1)
+    if spoil:                       # behind the last key
+        k[keys:] = math.nan
+        v[keys:] = math.inf
+    out = torch.full((rows, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((rows, heads), 7.0, device="cuda")
+    a = u.attn(q, out, lse, g if gate else None, kv_heads=kv_heads, scale=scale)
+    cq, ck = u.bounds(nq), u.bounds(nk)
+    dq, dk = u.ints(cq), u.ints(ck)
+    kk = B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), k_stride=k.stride(0), v_stride=v.stride(0),
+                    rows=keys + 9, cu_q=dq.data_ptr(), cu_k=dk.data_ptr(), seqs=len(nq),
+                    causal=int(causal))
+    gpu.attn_prompt_dev(a, kk, stream=u.stream())
+    torch.cuda.synchronize()
+    assert gpu.last_block_status() == 0
+    for i in range(len(nq)):
+        n, m = nq[i], nk[i]
+        limit = torch.full((n,), m, device="cuda")
+        if causal:
+            limit = (m - n + 1 + torch.arange(n, device="cuda")).clamp(min=0)
+        qs, ks = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
+        ref = u.exact(q[qs], k[ks], v[ks], limit, a.scale, g[qs] if gate else None)
+        u.check(out[qs], lse[qs], ref, (i, n, m))
+    assert (out[sum(nq):] == 7).all() and (lse[sum(nq):] == 7).all()
+    return out, lse
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_packed(gpu, heads, kv_heads, dim, causal):
+    import torch
+    n = [1, 16, 130, 0, 77, 257]
+    _prompt(gpu, torch, n, n, heads, kv_heads, dim, causal, pad=3)
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 700])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_one(gpu, n, dim):
+    import torch
+    _prompt(gpu, torch, [n], [n], 8, 1, dim, gate=False, seed=n)
+
+
+@pytest.mark.parametrize("nq,nk", [([1], [1000]), ([5, 40], [133, 900]), ([100], [0]),
+                                   ([200, 3], [150, 3]), ([0, 0], [5, 0]), ([300], [1])])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 2, 128), (4, 4, 64)])
+def test_prompt_keys_before_and_missing(gpu, nq, nk, heads, kv_heads, dim):
+    import torch
+    _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, seed=3)
+    _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, causal=False, seed=4)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_many_items(gpu, dim):
+    """More tiles than SMs, lengths from one token to many."""
+    import torch
+    n = [1 + (i * 37) % 400 for i in range(60)] + [1500, 1, 2]
+    _prompt(gpu, torch, n, n, 8, 4, dim, pad=100)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_large_scores(gpu, dim):
+    """Scores in the hundreds, rising along the row: the running maximum moves far."""
+    import torch
+    _prompt(gpu, torch, [600], [600], 4, 1, dim, scale=2.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_rising_keys(gpu, dim):
+    """Every later block of keys scores higher than all before: what has been summed has to be
+    scaled down again and again."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    n, H = 1024, 4
+    q = torch.zeros(n, H, dim, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 8.0
+    k = u.normal(n, 1, dim, seed=2)
+    k[:, 0, 0] = (torch.arange(n, device="cuda") // 16).bfloat16()
+    v = u.normal(n, 1, dim, seed=3)
+    out = torch.empty_like(q)
+    lse = torch.empty(n, H, device="cuda")
+    a = u.attn(q, out, lse, kv_heads=1, scale=0.25)
+    cu = u.ints([0, n])
+    kk = B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=n, cu_q=cu.data_ptr(),
+                    cu_k=cu.data_ptr(), seqs=1, causal=1)
+    gpu.attn_prompt_dev(a, kk, stream=u.stream())
+    torch.cuda.synchronize()
+    ref = u.exact(q, k, v, torch.arange(1, n + 1, device="cuda"), 0.25)
+    u.check(out, lse, ref)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 8, 128), (8, 1, 64)])
+def test_prompt_not_finite_where_nothing_sees(gpu, heads, kv_heads, dim):
+    """NaN and infinity behind the last key, and in the sequences beside a sound one."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    _prompt(gpu, torch, [50, 100], [50, 100], heads, kv_heads, dim, spoil=True)
+    n = [33, 90, 41]
+    cu = u.bounds(n)
+    q, k, v = (u.normal(sum(n), h, dim, seed=i) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    for t in (k, v):
+        t[:cu[1]] = math.nan
+        t[cu[2]:] = math.inf
+    q[cu[2]:] = math.nan
+    out = torch.empty_like(q)
+    a = u.attn(q, out, kv_heads=kv_heads)
+    d = u.ints(cu)
+    kk = B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=sum(n), cu_q=d.data_ptr(),
+                    cu_k=d.data_ptr(), seqs=3, causal=1)
+    gpu.attn_prompt_dev(a, kk, stream=u.stream())
+    torch.cuda.synchronize()
+    s = slice(cu[1], cu[2])
+    ref = u.exact(q[s], k[s], v[s], torch.arange(1, n[1] + 1, device="cuda"), a.scale)
+    u.check(out[s], None, ref)
+
+
+def _decode(gpu, torch, lengths, heads, kv_heads, dim, page, gate=True, seq=None, layers=1,
+            seed=0, scale=None, width=None):
+    import attn_util as u
+    held = [-(-n // page) for n in lengths]
+    cache = u.Cache(layers, sum(held) + 3, kv_heads, page, dim, len(lengths),
+                    width or max(held) + 2, seed).hold(lengths, seed)
+    # nothing behind a sequence's last token may matter
+    inside = torch.zeros(cache.pages, page, dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lengths):
+        t = torch.arange(n, device="cuda")
+        inside[cache.table[s, (t // page)].long(), t % page] = True
+    cache.k.transpose(2, 3)[:, ~inside] = math.nan
+    cache.v.transpose(2, 3)[:, ~inside] = math.inf
+    order = list(range(len(lengths))) if seq is None else seq
+    q, g = u.normal(len(order), 2, heads, dim, seed=seed + 5, scale=1.5).unbind(1)
+    out = torch.full((len(order), heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((len(order), heads), 7.0, device="cuda")
+    a = u.attn(q, out, lse, g if gate else None, kv_heads=kv_heads, scale=scale)
+    d = u.ints(order) if seq is not None else None
+    gpu.attn_decode_dev(a, cache.c, layers - 1, d.data_ptr() if seq is not None else None,
+                        stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 0
+    for b, s in enumerate(order):
+        if s < 0:
+            assert (out[b] == 7).all() and (lse[b] == 7).all()
+            continue
+        k, v = cache.tokens(layers - 1, s)
+        ref = u.exact(q[b:b + 1], k, v, u.ints([lengths[s]]), a.scale,
+                      g[b:b + 1] if gate else None)
+        u.check(out[b:b + 1], lse[b:b + 1], ref, (b, s, lengths[s]))
+    return a, cache, q, g, out, lse, d
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("page", [16, 32, 48, 256])
+def test_decode_lengths(gpu, heads, kv_heads, dim, page):
+    import torch
+    _decode(gpu, torch, [1, 15, 16, 17, 0, 31, 64, 65, 127, 300, 1023], heads, kv_heads, dim, page)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+def test_decode_long(gpu, heads, kv_heads, dim):
+    """One sequence over all SMs; two of very different lengths."""
+    import torch
+    _decode(gpu, torch, [20011], heads, kv_heads, dim, 64, gate=False, seed=1)
+    _decode(gpu, torch, [9000, 3], heads, kv_heads, dim, 16, seed=2)
+
+
+def test_decode_many_sequences(gpu):
+    import torch
+    n = [(i * 131) % 900 for i in range(333)]
+    _decode(gpu, torch, n, 8, 2, 128, 32)
+
+
+def test_decode_more_rows_than_a_launch_takes(gpu):
+    import torch
+    n = [(i * 7) % 40 for i in range(2600)]
+    _decode(gpu, torch, n, 4, 2, 64, 16, gate=False)
+
+
+def test_decode_order_padding_and_repeats(gpu):
+    """Rows in another order than the table, rows of no sequence, one sequence twice."""
+    import torch
+    _decode(gpu, torch, [40, 500, 0, 7], 16, 2, 256, 32, seq=[3, -1, 0, 1, 1, 2, -1, 0], layers=3)
+
+
+def test_decode_large_scores(gpu):
+    import torch
+    _decode(gpu, torch, [700, 33], 16, 2, 256, 32, scale=2.0)
+
+
+def test_decode_bad_pages_and_sequences(gpu):
+    """A page number outside of the pool: its tokens are left out, the status says so.  A
+    sequence that there is not: its row stays as it is."""
+    import torch
+    import attn_util as u
+    a, cache, q, g, out, lse, d = _decode(gpu, torch, [100, 200], 8, 2, 128, 32)
+    k, v = cache.tokens(0, 1)
+    cache.table[1, 2] = cache.pages
+    out.fill_(7.0)
+    gpu.attn_decode_dev(a, cache.c, 0, None, stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 3
+    kept = torch.cat([torch.arange(64), torch.arange(96, 200)]).cuda()
+    ref = u.exact(q[1:], k[kept], v[kept], u.ints([168]), a.scale, g[1:])
+    u.check(out[1:], lse[1:], ref)
+    cache.work[0] = 0
+    out.fill_(7.0)
+    seq = u.ints([5, 0])
+    gpu.attn_decode_dev(a, cache.c, 0, seq.data_ptr(), stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 2 and (out[0] == 7).all() and not (out[1] == 7).any()
+
+
+def test_decode_far_into_a_large_pool(gpu):
+    """Elements behind 2^31 of the pool."""
+    import torch
+    import attn_util as u
+    pages, page, K, D = 17000, 256, 2, 256
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("not enough memory")
+    k = torch.zeros(1, pages, K, page, D, dtype=torch.bfloat16, device="cuda")
+    cache = u.Cache(1, 1, K, page, D, 1, 4)
+    cache.refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    cache.work = torch.zeros(4 * pages + 100, dtype=torch.int32, device="cuda")
+    use = [16999, 0, 16998]
+    for i, p in enumerate(use):
+        k[0, p] = u.normal(K, page, D, seed=i)
+    cache.k = cache.v = k
+    cache.table[0, :3] = u.ints(use)
+    cache.len[0] = 700
+    c = cache.c
+    c.k = c.v = k.data_ptr()
+    c.refs, c.work, c.pages = cache.refs.data_ptr(), cache.work.data_ptr(), pages
+    q = u.normal(1, 16, D, seed=9)
+    out = torch.empty_like(q)
+    a = u.attn(q, out, kv_heads=K)
+    gpu.attn_decode_dev(a, c, 0, None, stream=u.stream())
+    torch.cuda.synchronize()
+    kk, vv = cache.tokens(0, 0)
+    u.check(out, None, u.exact(q, kk, vv, u.ints([700]), a.scale))
+
+
+def test_same_result_twice_on_streams_and_in_a_graph(gpu):
+    """Bit for bit the same: called again, called on two streams at once, replayed from a graph
+    after the inputs have changed."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    a, cache, q, g, out, lse, d = _decode(gpu, torch, [3000, 40, 777], 16, 2, 256, 64, seed=4)
+    n = [300, 45]
+    pq, pk, pv = (u.normal(sum(n), h, 256, seed=i) for i, h in enumerate((16, 2, 2)))
+    pout = torch.empty_like(pq)
+    cu = u.ints(u.bounds(n))
+    pa = u.attn(pq, pout, kv_heads=2)
+    kk = B.AttnKeys(k=pk.data_ptr(), v=pv.data_ptr(), rows=sum(n), cu_q=cu.data_ptr(),
+                    cu_k=cu.data_ptr(), seqs=2, causal=1)
+
+    def both(s):
+        gpu.attn_prompt_dev(pa, kk, stream=s)
+        gpu.attn_decode_dev(a, cache.c, 0, None, stream=s)
+
+    both(u.stream())
+    torch.cuda.synchronize()
+    first = out.clone(), lse.clone(), pout.clone()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        out.zero_()
+        pout.zero_()
+        torch.cuda.synchronize()
+        gpu.attn_decode_dev(a, cache.c, 0, None, stream=s1.cuda_stream)
+        gpu.attn_prompt_dev(pa, kk, stream=s2.cuda_stream)
+        gpu.attn_decode_dev(a, cache.c, 0, None, stream=s2.cuda_stream)
+        gpu.attn_prompt_dev(pa, kk, stream=s1.cuda_stream)
+        torch.cuda.synchronize()
+        for x, y in zip(first, (out, lse, pout)):
+            assert torch.equal(x, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both(u.stream())
+    old = q.clone(), pq.clone()
+    q.copy_(-q)
+    pq.copy_(-pq)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not torch.equal(first[0], out) and not torch.equal(first[2], pout)
+    q.copy_(old[0])
+    pq.copy_(old[1])
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(first, (out, lse, pout)):
+        assert torch.equal(x, y)
