@@ -32,8 +32,8 @@ static int kv_view(const ApusCudaKvCache *kv, const char *what, KvView *out) {
     if (!aligned16(kv->k) || !aligned16(kv->v))
         return fail("%s: the pools must be 16-byte aligned", what);
     const size_t most = 0x7fffffff;
-    if (kv->pages > most / kv->page_tokens || kv->max_pages > most / kv->page_tokens ||
-        kv->layers > 65536 || kv->kv_heads > 1024 || kv->seqs > most / 64 ||
+    if (kv->kv_heads > 1024 || kv->pages > most / (kv->page_tokens * kv->kv_heads) ||
+        kv->max_pages > most / kv->page_tokens || kv->layers > 65536 || kv->seqs > most / 64 ||
         kv->kv_heads * kv->page_tokens > most / kv->head_dim)
         return fail("%s: the cache is too large", what);
     KvView v;
@@ -273,13 +273,11 @@ static int attn_view(const ApusCudaAttn *a, const char *what, AttnView *out) {
     return 0;
 }
 
-template <bool PAGED>
-static int launch_rows(const AttnView &a, size_t D, const AttnPacked &pk, const AttnPaged &pg,
-                       cudaStream_t st) {
+static int launch_rows(const AttnView &a, size_t D, const AttnPacked &pk, cudaStream_t st) {
     const dim3 grid((unsigned)(((size_t)a.rows * a.heads + 7) / 8));
-    if (D == 64) LAUNCH_OK(launch_k(attn_rows_kernel<64, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
-    else if (D == 128) LAUNCH_OK(launch_k(attn_rows_kernel<128, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
-    else LAUNCH_OK(launch_k(attn_rows_kernel<256, PAGED>, grid, dim3(256), 0, st, a, pk, pg));
+    if (D == 64) LAUNCH_OK(launch_k(attn_rows_kernel<64>, grid, dim3(256), 0, st, a, pk));
+    else if (D == 128) LAUNCH_OK(launch_k(attn_rows_kernel<128>, grid, dim3(256), 0, st, a, pk));
+    else LAUNCH_OK(launch_k(attn_rows_kernel<256>, grid, dim3(256), 0, st, a, pk));
     return 0;
 }
 
@@ -313,38 +311,82 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     cudaStream_t st = (cudaStream_t)stream;
     Ordered ord(g_ctx, st);
     if (ord.rc) return 1;
-    return launch_rows<false>(v, a->head_dim, pk, AttnPaged{}, st);
+    return launch_rows(v, a->head_dim, pk, st);
+}
+
+/* rows of head_dim values, 16 tokens of 64 values at a time, 128B swizzle */
+static int decode_map(CUtensorMap *m, const uint16_t *base, size_t rows, size_t D) {
+    PFN_encodeTiled_local enc = tensor_map_encoder();
+    if (!enc) return fail("%s", prefill_last_error());
+    cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)(D / 64)};
+    cuuint64_t strides[2] = {(cuuint64_t)D * 2, 128};
+    cuuint32_t box[3] = {64, AD_TILE, (cuuint32_t)(D / 64)}, estr[3] = {1, 1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(base), dims,
+                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : fail("attn_decode_dev: cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+template <int D, int NH>
+static int launch_decode(Ctx *c, const CUtensorMap &mk, const CUtensorMap &mv, DecodeParams p,
+                         cudaStream_t st) {
+    const int smem = ad_smem_bytes(), grid = c->sm_count < AD_MAX_CTAS ? c->sm_count : AD_MAX_CTAS;
+    static bool set = false;
+    if (!set) {
+        CU_OK(cudaFuncSetAttribute(attn_decode_kernel<D, NH>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        set = true;
+    }
+    for (int row = 0; row < p.a.rows; row += AD_MAX_ROWS) {
+        p.row0 = row;
+        p.rows = p.a.rows - row < AD_MAX_ROWS ? p.a.rows - row : AD_MAX_ROWS;
+        LAUNCH_OK(launch_k(attn_decode_kernel<D, NH>, dim3(grid), dim3(AD_THREADS), smem, st, mk,
+                           mv, p));
+        LAUNCH_OK(launch_k(attn_join_kernel<D>, dim3(grid, p.a.group), dim3(D), 0, st, p, grid));
+    }
+    return 0;
 }
 
 extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv,
                                          size_t layer, const int32_t *d_seq, void *stream) {
     if (!a) return fail("attn_decode_dev: bad args");
-    AttnView v;
+    DecodeParams p = {};
     KvView c;
-    if (attn_view(a, "attn_decode_dev", &v)) return 1;
+    if (attn_view(a, "attn_decode_dev", &p.a)) return 1;
     if (kv_view(kv, "attn_decode_dev", &c)) return 1;
     if (kv->kv_heads != a->kv_heads || kv->head_dim != a->head_dim || layer >= kv->layers)
         return fail("attn_decode_dev: the cache has other heads or fewer layers");
     if (!d_seq && a->rows > kv->seqs) return fail("attn_decode_dev: more rows than sequences");
     if (!a->rows) return 0;
-    AttnPaged pg = {};
-    const size_t at = layer * kv->pages * (size_t)c.page_elems;
-    pg.k = kv->k + at;
-    pg.v = kv->v + at;
-    pg.table = kv->table;
-    pg.len = kv->len;
-    pg.seq = d_seq;
-    pg.status = kv->work;
-    pg.pages = c.pages;
-    pg.page_tokens = c.page_tokens;
-    pg.seqs = c.seqs;
-    pg.max_pages = c.max_pages;
-    pg.kv_heads = (int)kv->kv_heads;
+    p.table = kv->table;
+    p.len = kv->len;
+    p.seq = d_seq;
+    p.status = kv->work;
+    p.pages = c.pages;
+    p.page_tokens = c.page_tokens;
+    p.seqs = c.seqs;
+    p.max_pages = c.max_pages;
+    p.kv_heads = (int)kv->kv_heads;
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
-    DeviceGuard dev(g_ctx->device);
+    Ctx *x = g_ctx;
+    DeviceGuard dev(x->device);
+    CUtensorMap mk, mv;
+    const size_t D = kv->head_dim, at = layer * kv->pages * (size_t)c.page_elems;
+    const size_t rows = kv->pages * kv->kv_heads * kv->page_tokens;
+    if (decode_map(&mk, kv->k + at, rows, D) || decode_map(&mv, kv->v + at, rows, D)) return 1;
     cudaStream_t st = (cudaStream_t)stream;
-    Ordered ord(g_ctx, st);
+    Ordered ord(x, st);
     if (ord.rc) return 1;
-    return launch_rows<true>(v, a->head_dim, AttnPacked{}, pg, st);
+    p.wait_status = x->d_status;
+    p.parts = x->d_attn_parts;
+    p.items = x->d_attn_items;
+    const bool wide = p.a.group > 8;
+    if (D == 64) return wide ? launch_decode<64, 16>(x, mk, mv, p, st)
+                             : launch_decode<64, 8>(x, mk, mv, p, st);
+    if (D == 128) return wide ? launch_decode<128, 16>(x, mk, mv, p, st)
+                              : launch_decode<128, 8>(x, mk, mv, p, st);
+    return wide ? launch_decode<256, 16>(x, mk, mv, p, st)
+                : launch_decode<256, 8>(x, mk, mv, p, st);
 }

@@ -1,0 +1,582 @@
+/*
+ * attn_decode.cuh — attention of one new token a sequence over the pages of a cache.
+ *
+ *   s_j = scale q . k_j over all tokens j of the sequence,  p = softmax(s),
+ *   o = (sum_j p_j v_j) * sigmoid(gate),  lse = log sum_j exp(s_j)
+ *
+ * Bound: HBM, every key and value once: 4 * head_dim bytes a token and key head, against which
+ * the products of its heads (at most 16 queries a key) are small.  So the work is split over
+ * tokens, not heads: all sequences' tiles of 16 tokens form one line, (row, key head, tile), that
+ * is cut into as many equal pieces as there are warps (eight to an SM), whatever the lengths are.  A
+ * warp runs along its piece with a running maximum and sum, fed by a ring of its own in shared
+ * memory that TMA fills (24 KB a warp, 192 KB an SM, of which about 44 KB in flight would cover the
+ * latency), across the ends of sequences.  The heads of one key head are the rows (for the
+ * scores) and the columns (for the outputs) of mma.sync tiles of 8: what tcgen05 would do with
+ * 128 rows would be 8 or 16 rows here, and mma.sync needs a fifth of its rate to keep up with HBM.
+ *
+ *   scores   S[heads x 16 tokens] = Q . K^T       A: q in registers, B: ldmatrix of K
+ *   outputs  O^T[D x heads] += V^T . P^T          A: ldmatrix.trans of V, B: the scores'
+ *                                                 accumulators as they lie, narrowed to BF16
+ *
+ * A piece that holds a sequence's tokens only in part leaves (max, sum, outputs) behind: those of
+ * one SM are put together in shared memory, those of several SMs by attn_join_kernel, always in
+ * the order of the line, so that a result does not depend on timing.
+ */
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attn_view.cuh"
+#include "common.cuh"
+#include "kv_pages.cuh"
+#include "prefill_gemm.cuh"
+
+namespace apus {
+
+constexpr int AD_WARPS = 8;
+constexpr int AD_THREADS = AD_WARPS * 32;
+constexpr int AD_TILE = 16;                  /* tokens */
+constexpr int AD_MAX_ROWS = 1024;            /* of a launch */
+constexpr int AD_RING_BYTES = 24 << 10;      /* of a warp */
+constexpr int AD_MAX_CTAS = 256;
+constexpr int AD_MAX_GROUP = 16;
+constexpr int AD_MAX_DIM = 256;
+/* one unfinished result: outputs, then max and sum of each head */
+constexpr int AD_PART_FLOATS = AD_MAX_GROUP * AD_MAX_DIM + 2 * AD_MAX_GROUP;
+
+struct DecodeParams {
+    AttnView a;
+    const int32_t *table, *len, *seq;
+    int32_t *status;                         /* the cache's */
+    int *wait_status;                        /* the library's */
+    int pages, page_tokens, seqs, max_pages, kv_heads;
+    int row0, rows;                          /* of this launch */
+    /* [gridDim][2] parts of this launch's CTAs: 0 began in an earlier CTA, 1 goes on in a later one;
+     * then one for each warp: what ends in it and began in an earlier one */
+    float *parts;
+    int *items;                              /* [gridDim][2] whose they are, -1: none */
+};
+
+inline size_t ad_scratch_floats(int sms) {
+    return (size_t)sms * (2 + AD_WARPS) * AD_PART_FLOATS;
+}
+
+template <int D>
+struct AdShape {
+    static constexpr int TILE_BYTES = AD_TILE * D * 2;
+    static constexpr int STAGES = AD_RING_BYTES / TILE_BYTES;       /* 3, 6, 12 */
+};
+
+struct AdShared {
+    long long start[AD_MAX_ROWS + 1];        /* tiles before a row */
+    int seq[AD_MAX_ROWS], len[AD_MAX_ROWS];
+    uint64_t full[AD_WARPS][12];
+    int valid[AD_WARPS][12];                 /* tokens of a stage that count */
+    float m[AD_WARPS][2][AD_MAX_GROUP], l[AD_WARPS][2][AD_MAX_GROUP];
+    int item[AD_WARPS][2];
+    long long scan[AD_WARPS];
+};
+inline int ad_smem_bytes() { return AD_WARPS * AD_RING_BYTES + (int)sizeof(AdShared) + 1024; }
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                            int z, uint64_t *bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
+        "complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z),
+        "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+/* where a warp is on the line */
+struct AdCursor {
+    int row, head, tile, tiles;              /* tiles: of the row */
+    __device__ __forceinline__ void seek(const AdShared &s, int rows, int kv_heads,
+                                         long long at) {
+        int lo = 0, hi = rows;               /* the last row that starts at or before it */
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s.start[mid] * kv_heads <= at) lo = mid;
+            else hi = mid;
+        }
+        row = lo;
+        tiles = (int)(s.start[row + 1] - s.start[row]);
+        const long long in = at - s.start[row] * kv_heads;
+        head = tiles ? (int)(in / tiles) : 0;
+        tile = tiles ? (int)(in - (long long)head * tiles) : 0;
+    }
+    __device__ __forceinline__ void next_item(const AdShared &s, int rows, int kv_heads) {
+        tile = 0;
+        if (++head < kv_heads) return;
+        head = 0;
+        do
+            row++;
+        while (row < rows && s.start[row + 1] == s.start[row]);
+        tiles = row < rows ? (int)(s.start[row + 1] - s.start[row]) : 0;
+    }
+};
+
+/* o of one head, narrowed once: gate included */
+__device__ __forceinline__ uint16_t ad_out(const AttnView &a, long row, int at, float y) {
+    if (a.gate) y *= sigmoid_f32(bf16_f32(a.gate[row * a.gate_stride + at]));
+    return bf16_bits(y);
+}
+
+template <int D, int NH>
+__global__ void __launch_bounds__(AD_THREADS, 1)
+attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v,
+                   const __grid_constant__ DecodeParams p) {
+    constexpr int STAGES = AdShape<D>::STAGES, TILE_BYTES = AdShape<D>::TILE_BYTES;
+    constexpr int MT = D / 16;                            /* row tiles of O^T, steps of Q . K^T */
+    constexpr int NT = NH / 8;                            /* column tiles of O^T */
+    extern __shared__ unsigned char ad_raw[];
+    unsigned char *ring0 = reinterpret_cast<unsigned char *>(
+        (reinterpret_cast<uintptr_t>(ad_raw) + 1023) & ~(uintptr_t)1023);
+    AdShared &s = *reinterpret_cast<AdShared *>(ring0 + AD_WARPS * AD_RING_BYTES);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const int group = p.a.group;
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; i++) mbar_init(&s.full[warp][i], 1);
+        mbar_fence_init();
+    }
+    pdl_enter();
+
+    /* ---- the line: tiles before every row (each CTA for itself) ---- */
+    {
+        constexpr int PER = AD_MAX_ROWS / AD_THREADS;
+        long long mine[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int r = tid * PER + i;
+            int q = -1, n = 0;
+            if (r < p.rows) {
+                q = p.seq ? p.seq[p.row0 + r] : p.row0 + r;
+                if (q >= p.seqs) {
+                    if (blockIdx.x == 0) atomicCAS(p.status, 0, KV_BAD_LIST);
+                    q = -1;
+                }
+                if (q >= 0) n = min(max(p.len[q], 0), p.max_pages * p.page_tokens);
+                s.seq[r] = q;
+                s.len[r] = n;
+            }
+            mine[i] = sum;
+            sum += (n + AD_TILE - 1) / AD_TILE;
+        }
+        long long x = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s.scan[warp] = x;
+        __syncthreads();
+        long long before = x - sum;
+        for (int w = 0; w < warp; w++) before += s.scan[w];
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (tid * PER + i <= p.rows) s.start[tid * PER + i] = before + mine[i];
+        if (tid == AD_THREADS - 1 && p.rows == AD_MAX_ROWS) s.start[p.rows] = before + sum;
+        if (tid < 2 * AD_WARPS) s.item[tid >> 1][tid & 1] = -1;
+    }
+    __syncthreads();
+    const long long total = s.start[p.rows] * p.kv_heads;
+    long long per = (total + gridDim.x - 1) / gridDim.x;
+    if (per < AD_WARPS) per = AD_WARPS;                   /* one tile to a warp */
+    const long long lo = min(total, per * blockIdx.x), hi = min(total, lo + per);
+    const long long from = lo + (hi - lo) * warp / AD_WARPS,
+                    to = lo + (hi - lo) * (warp + 1) / AD_WARPS;
+
+    /* rows of no token: zeros */
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        if (s.seq[r] < 0 || s.len[r] > 0) continue;
+        const long row = p.row0 + r;
+        for (int i = tid; i < p.a.heads * D; i += AD_THREADS)
+            p.a.out[row * p.a.out_stride + i] = 0;
+        if (p.a.lse)
+            for (int h = tid; h < p.a.heads; h += AD_THREADS)
+                p.a.lse[row * p.a.heads + h] = -INFINITY;
+    }
+
+    /* ---- the warp's piece ---- */
+    const uint32_t ring = smem_u32(ring0) + warp * AD_RING_BYTES;
+    const float sc = p.a.scale * LOG2E;
+    const uint64_t policy = l2_read_once();
+    bool alive = true;
+    float o[NT][MT][4], m[NT], l[NT];
+    uint32_t qa[MT][NT * 2];
+    long long issued = from, done = from;                 /* tiles asked for, tiles summed */
+    AdCursor ci, cc;
+    ci.seek(s, p.rows, p.kv_heads, from);
+    cc = ci;
+    /* copies: the keys of tile i are copy 2i, its values 2i + 1, each into stage copy % STAGES */
+    uint32_t copies = 0, used = 0;
+    int page_row = -1, page_base = 0, page_lane = 0;      /* pages of 32 tiles, one to a lane */
+    int coord = 0, count = 0;
+    auto issue = [&]() {
+        const int st = (int)(copies % STAGES);
+        const bool keys = !(copies & 1);
+        if (keys) {
+            if (page_row != ci.row || ci.tile < page_base || ci.tile >= page_base + 32) {
+                page_row = ci.row;
+                page_base = ci.tile;
+                const int tile = page_base + lane;
+                page_lane = tile < ci.tiles
+                                ? p.table[(size_t)s.seq[ci.row] * p.max_pages +
+                                          (unsigned)(tile * AD_TILE) / (unsigned)p.page_tokens]
+                                : 0;
+            }
+            int page = __shfl_sync(0xffffffffu, page_lane, ci.tile - page_base);
+            count = min(AD_TILE, s.len[ci.row] - ci.tile * AD_TILE);
+            if ((unsigned)page >= (unsigned)p.pages) {
+                if (lane == 0) atomicCAS(p.status, 0, KV_BAD_PAGE);
+                page = 0;
+                count = 0;
+            }
+            coord = (page * p.kv_heads + ci.head) * p.page_tokens +
+                    (int)((unsigned)(ci.tile * AD_TILE) % (unsigned)p.page_tokens);
+        }
+        if (lane == 0) {
+            s.valid[warp][st] = count;
+            mbar_expect_tx(&s.full[warp][st], TILE_BYTES);
+            tma_load_3d(ring + st * TILE_BYTES, keys ? &map_k : &map_v, 0, coord, 0,
+                        &s.full[warp][st], policy);
+        }
+        copies++;
+        if (!keys) {
+            issued++;
+            if (++ci.tile == ci.tiles) ci.next_item(s, p.rows, p.kv_heads);
+        }
+    };
+    while (copies < STAGES && issued < to) issue();
+
+    auto begin = [&]() {                                  /* q of the item's heads, nothing summed */
+        const long row = p.row0 + cc.row;
+        const uint16_t *q = p.a.q + row * p.a.q_stride + (size_t)cc.head * group * D;
+#pragma unroll
+        for (int k = 0; k < MT; k++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    qa[k][n * 2 + j] =
+                        g + 8 * n < group ? *reinterpret_cast<const uint32_t *>(
+                                                q + (g + 8 * n) * D + k * 16 + j * 8 + t4 * 2)
+                                          : 0u;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < MT; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[n][k][j] = 0.0f;
+        }
+    };
+    /* an unfinished result in fp32: [group][D] */
+    auto leave = [&](float *dst, int slot) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int h = n * 8 + t4 * 2 + (j & 1);
+                if (h < group)
+#pragma unroll
+                    for (int k = 0; k < MT; k++)
+                        dst[h * D + k * 16 + (j >> 1) * 8 + g] = o[n][k][j];
+            }
+            if (t4 == 0) {
+                s.m[warp][slot][n * 8 + g] = m[n];
+                s.l[warp][slot][n * 8 + g] = l[n];
+            }
+        }
+    };
+    const size_t warp_part =
+        (size_t)(2 * gridDim.x + blockIdx.x * AD_WARPS + warp) * AD_PART_FLOATS;
+    bool first = cc.tile > 0;              /* the item began before this piece */
+    if (from < to) begin();
+    while (alive && done < to) {
+        /* ---- scores of 16 tokens ---- */
+        int st = (int)(used % STAGES);
+        if (!mbar_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
+            alive = false;
+            break;
+        }
+        const int valid = s.valid[warp][st];
+        float sc0[NT][2], sc1[NT][2];                     /* [head tile][token pair] by token tile */
+        {
+            float c[2][4] = {};
+            const uint32_t base = ring + st * TILE_BYTES;
+            const int tok = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
+#pragma unroll
+            for (int k = 0; k < MT; k++) {
+                uint32_t b[4];
+                const int chunk = (2 * k + ch) & 7;
+                ldmatrix_x4(b, base + (k >> 2) * (AD_TILE * 128) + tok * 128 +
+                                   ((chunk ^ (tok & 7)) << 4));
+                const uint32_t a[4] = {qa[k][0], NT > 1 ? qa[k][2 * (NT - 1)] : 0u, qa[k][1],
+                                       NT > 1 ? qa[k][2 * (NT - 1) + 1] : 0u};
+                mma_16x8(c[0], a, b[0], b[1]);
+                mma_16x8(c[1], a, b[2], b[3]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    sc0[n][j] = t4 * 2 + j < valid ? c[0][n * 2 + j] * sc : -INFINITY;
+                    sc1[n][j] = 8 + t4 * 2 + j < valid ? c[1][n * 2 + j] * sc : -INFINITY;
+                }
+        }
+        used++;
+        __syncwarp();
+        if (issued < to) issue();
+        /* ---- running maximum; what has been summed is scaled down only where the maximum
+         * has moved by more than 2^8, which fp32 sums and BF16 weights of any size bear ---- */
+        float f[NT];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float x = fmaxf(fmaxf(sc0[n][0], sc0[n][1]), fmaxf(sc1[n][0], sc1[n][1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            f[n] = 1.0f;
+            if (x > m[n] + 8.0f || (m[n] == -INFINITY && x > -INFINITY)) {
+                f[n] = exp2_fast(m[n] - x);
+                m[n] = x;
+                l[n] *= f[n];
+                moved = true;
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float f0 = __shfl_sync(0xffffffffu, f[n], t4 * 8),
+                            f1 = __shfl_sync(0xffffffffu, f[n], t4 * 8 + 4);
+#pragma unroll
+                for (int k = 0; k < MT; k++) {
+                    o[n][k][0] *= f0;
+                    o[n][k][1] *= f1;
+                    o[n][k][2] *= f0;
+                    o[n][k][3] *= f1;
+                }
+            }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float mm = m[n] == -INFINITY ? 0.0f : m[n];
+            const float p0 = exp2_fast(sc0[n][0] - mm), p1 = exp2_fast(sc0[n][1] - mm),
+                        p2 = exp2_fast(sc1[n][0] - mm), p3 = exp2_fast(sc1[n][1] - mm);
+            l[n] += (p0 + p1) + (p2 + p3);
+            pb[n][0] = pack_bf16_rn(p0, p1);
+            pb[n][1] = pack_bf16_rn(p2, p3);
+        }
+        /* ---- outputs ---- */
+        st = (int)(used % STAGES);
+        if (!mbar_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
+            alive = false;
+            break;
+        }
+        {
+            const uint32_t base = ring + st * TILE_BYTES;
+            const int tok = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
+            /* values of tokens that do not count may be anything: 0 * NaN is not 0 */
+            const uint32_t keep0 = (t4 * 2 < valid ? 0xffffu : 0u) |
+                                   (t4 * 2 + 1 < valid ? 0xffff0000u : 0u),
+                           keep1 = (8 + t4 * 2 < valid ? 0xffffu : 0u) |
+                                   (8 + t4 * 2 + 1 < valid ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int k = 0; k < MT; k++) {
+                uint32_t a[4];
+                const int chunk = (2 * k + ch) & 7;
+                ldmatrix_x4_trans(a, base + (k >> 2) * (AD_TILE * 128) + tok * 128 +
+                                         ((chunk ^ (tok & 7)) << 4));
+                a[0] &= keep0;
+                a[1] &= keep0;
+                a[2] &= keep1;
+                a[3] &= keep1;
+#pragma unroll
+                for (int n = 0; n < NT; n++) mma_16x8(o[n][k], a, pb[n][0], pb[n][1]);
+            }
+        }
+        used++;
+        __syncwarp();
+        if (issued < to) issue();
+        done++;
+        const bool ends = ++cc.tile == cc.tiles;
+        if (!ends && done < to) continue;
+        /* ---- the end of the item or of the piece ---- */
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+        }
+        const int item = cc.row * p.kv_heads + cc.head;
+        if (ends && !first) {                             /* all of it was here */
+            const long row = p.row0 + cc.row;
+            const int h0 = cc.head * group;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float inv = l[n] > 0.0f ? __fdividef(1.0f, l[n]) : 0.0f;
+                if (p.a.lse && t4 == 0 && n * 8 + g < group)
+                    p.a.lse[row * p.a.heads + h0 + n * 8 + g] =
+                        l[n] > 0.0f ? (m[n] + log2f(l[n])) * LN2 : -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float v = __shfl_sync(0xffffffffu, inv, t4 * 8 + j * 4);
+                    const int h = n * 8 + t4 * 2 + j;
+                    if (h < group) {
+#pragma unroll
+                        for (int k = 0; k < MT; k++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const int at = (h0 + h) * D + k * 16 + i * 8 + g;
+                                p.a.out[row * p.a.out_stride + at] =
+                                    ad_out(p.a, row, at, o[n][k][i * 2 + j] * v);
+                            }
+                    }
+                }
+            }
+        } else if (done == to) {                          /* in the ring, once all is through */
+            if (lane == 0) s.item[warp][1] = item;
+        } else {                                          /* out of the way of what comes */
+            leave(p.parts + warp_part, 0);
+            if (lane == 0) s.item[warp][0] = item;
+        }
+        first = false;
+        if (done < to) {
+            cc.next_item(s, p.rows, p.kv_heads);
+            begin();
+        }
+    }
+    if (!alive) {                                         /* a copy never came: no result, no hang */
+        if (lane == 0) set_status(p.wait_status, ST_MBAR_TIMEOUT);
+        for (; used < copies; used++)
+            mbar_wait(&s.full[warp][used % STAGES], (used / STAGES) & 1u);
+    }
+    __syncthreads();                                      /* every ring is read to its end */
+    float *mine = reinterpret_cast<float *>(ring0) + warp * (AD_RING_BYTES / 4);
+    if (s.item[warp][1] >= 0) leave(mine, 1);
+    __syncthreads();
+
+    /* ---- the SM's unfinished results, put together in the order of the line ---- */
+    if (tid < 2) p.items[blockIdx.x * 2 + tid] = -1;
+    __syncthreads();
+    for (int e = 0; e < 2 * AD_WARPS;) {
+        const int item = s.item[e >> 1][e & 1];
+        if (item < 0) {
+            e++;
+            continue;
+        }
+        int end = e + 1;                                  /* entries of the same item */
+        while (end < 2 * AD_WARPS && (s.item[end >> 1][end & 1] == item ||
+                                      s.item[end >> 1][end & 1] < 0))
+            end++;
+        const int r = item / p.kv_heads, kh = item - r * p.kv_heads;
+        const long long begin_at =
+            s.start[r] * p.kv_heads + (long long)kh * (s.start[r + 1] - s.start[r]);
+        const long long end_at = begin_at + (s.start[r + 1] - s.start[r]);
+        const bool before = begin_at < lo, after = end_at > hi;
+        const long row = p.row0 + r;
+        float *part = p.parts + (size_t)(blockIdx.x * 2 + (before ? 0 : 1)) * AD_PART_FLOATS;
+        for (int i = tid; i < group * D; i += AD_THREADS) {
+            const int h = i / D;
+            float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+            for (int j = e; j < end; j++)
+                if (s.item[j >> 1][j & 1] >= 0) top = fmaxf(top, s.m[j >> 1][j & 1][h]);
+            for (int j = e; j < end; j++) {
+                const int w = j >> 1;
+                if (s.item[w][j & 1] < 0 || s.m[w][j & 1][h] == -INFINITY) continue;
+                const float f = exp2_fast(s.m[w][j & 1][h] - top);
+                const float *src =
+                    j & 1 ? reinterpret_cast<float *>(ring0) + w * (AD_RING_BYTES / 4)
+                          : p.parts + (size_t)(2 * gridDim.x + blockIdx.x * AD_WARPS + w) *
+                                          AD_PART_FLOATS;
+                sum = fmaf(f, s.l[w][j & 1][h], sum);
+                acc = fmaf(f, src[i], acc);
+            }
+            if (before || after) {
+                part[i] = acc;
+                if (i % D == 0) {
+                    part[AD_MAX_GROUP * AD_MAX_DIM + h] = top;
+                    part[AD_MAX_GROUP * AD_MAX_DIM + AD_MAX_GROUP + h] = sum;
+                }
+            } else {
+                const int at = kh * group * D + i;
+                p.a.out[row * p.a.out_stride + at] =
+                    ad_out(p.a, row, at, sum > 0.0f ? __fdividef(acc, sum) : 0.0f);
+                if (p.a.lse && i % D == 0)
+                    p.a.lse[row * p.a.heads + kh * group + h] =
+                        sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+            }
+        }
+        if (tid == 0 && (before || after)) p.items[blockIdx.x * 2 + (before ? 0 : 1)] = item;
+        e = end;
+    }
+}
+
+/* An item that several SMs hold parts of begins in one of them: a CTA for each SM and head looks
+ * whether one begins there, and adds up its parts in order. */
+template <int D>
+__global__ void __launch_bounds__(D) attn_join_kernel(const __grid_constant__ DecodeParams p,
+                                                      int ctas) {
+    pdl_enter();
+    const int c = blockIdx.x, h = blockIdx.y, i = threadIdx.x, group = p.a.group;
+    const int item = p.items[c * 2 + 1];
+    if (item < 0) return;
+    __shared__ int s_end;
+    __shared__ float weight[AD_MAX_CTAS], sums[AD_MAX_CTAS];
+    if (i == 0) s_end = ctas;
+    __syncthreads();
+    for (int e = c + 1 + i; e < ctas; e += D)
+        if (p.items[e * 2] != item) {
+            atomicMin(&s_end, e);
+            break;
+        }
+    __syncthreads();
+    const int end = s_end;
+    auto part = [&](int e) {
+        return p.parts + (size_t)(e * 2 + (e == c ? 1 : 0)) * AD_PART_FLOATS;
+    };
+    constexpr int ML = AD_MAX_GROUP * AD_MAX_DIM;
+    const int parts = end - c;
+    for (int e = i; e < parts; e += D) {
+        weight[e] = part(c + e)[ML + h];
+        sums[e] = part(c + e)[ML + AD_MAX_GROUP + h];
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+    for (int e = 0; e < parts; e++) top = fmaxf(top, weight[e]);
+    if (top == -INFINITY) top = 0.0f;                     /* nothing counted: weights of 0 */
+    __syncthreads();
+    for (int e = i; e < parts; e += D) weight[e] = exp2_fast(weight[e] - top);
+    __syncthreads();
+#pragma unroll 16
+    for (int e = 0; e < parts; e++) {
+        sum = fmaf(weight[e], sums[e], sum);
+        acc = fmaf(weight[e], part(c + e)[h * D + i], acc);
+    }
+    const int r = item / p.kv_heads, kh = item - r * p.kv_heads;
+    const long row = p.row0 + r;
+    const int at = (kh * group + h) * D + i;
+    p.a.out[row * p.a.out_stride + at] =
+        ad_out(p.a, row, at, sum > 0.0f ? __fdividef(acc, sum) : 0.0f);
+    if (p.a.lse && i == 0)
+        p.a.lse[row * p.a.heads + kh * group + h] =
+            sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+}
+
+}  // namespace apus

@@ -1,6 +1,5 @@
 /*
- * attn_rows.cuh — attention of one row and head by one warp, over packed keys or over the pages
- * of a cache: the plainest form of
+ * attn_rows.cuh — attention of one row and head by one warp, over packed keys: the plainest form of
  *     s_j = scale q . k_j,   p = softmax(s),   o = sum_j p_j v_j,   lse = log sum_j exp(s_j)
  * with a running maximum and sum.
  */
@@ -8,19 +7,11 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "attn_view.cuh"
 #include "common.cuh"
 #include "kv_pages.cuh"
 
 namespace apus {
-
-struct AttnView {
-    const uint16_t *q, *gate;
-    uint16_t *out;
-    float *lse;
-    long q_stride, gate_stride, out_stride;
-    int rows, heads, group;
-    float scale;
-};
 
 struct AttnPacked {
     const uint16_t *k, *v;
@@ -29,29 +20,17 @@ struct AttnPacked {
     int rows, seqs, causal;
 };
 
-struct AttnPaged {
-    const uint16_t *k, *v;                     /* of the layer */
-    const int32_t *table, *len, *seq;
-    int32_t *status;
-    int pages, page_tokens, seqs, max_pages, kv_heads;
-};
-
-template <int D, bool PAGED>
+template <int D>
 __global__ void __launch_bounds__(256)
-attn_rows_kernel(AttnView a, AttnPacked pk, AttnPaged pg) {
+attn_rows_kernel(AttnView a, AttnPacked pk) {
     pdl_enter();
     constexpr int N = D / 32;
     const int lane = threadIdx.x & 31;
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= (long)a.rows * a.heads) return;
     const int row = (int)(item / a.heads), h = (int)(item % a.heads), kh = h / a.group;
-    int begin = 0, count = 0, s = 0;
-    if (PAGED) {
-        s = pg.seq ? pg.seq[row] : row;
-        if (s >= pg.seqs) atomicCAS(pg.status, 0, KV_BAD_LIST);
-        if (s < 0 || s >= pg.seqs) return;
-        count = max(0, min(pg.len[s], pg.max_pages * pg.page_tokens));
-    } else {
+    int begin, count;
+    {
         int lo = 0, hi = pk.seqs;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -72,21 +51,8 @@ attn_rows_kernel(AttnView a, AttnPacked pk, AttnPaged pg) {
     }
     float m = -INFINITY, l = 0.0f;
     for (int j = 0; j < count; j++) {
-        const uint16_t *k, *v;
-        if (PAGED) {
-            const int page = pg.table[(size_t)s * pg.max_pages + j / pg.page_tokens];
-            if ((unsigned)page >= (unsigned)pg.pages) {
-                atomicCAS(pg.status, 0, KV_BAD_PAGE);
-                continue;
-            }
-            const size_t at = (((size_t)page * pg.kv_heads + kh) * pg.page_tokens +
-                               j % pg.page_tokens) * D;
-            k = pg.k + at;
-            v = pg.v + at;
-        } else {
-            k = pk.k + (size_t)(begin + j) * pk.k_stride + kh * D;
-            v = pk.v + (size_t)(begin + j) * pk.v_stride + kh * D;
-        }
+        const uint16_t *k = pk.k + (size_t)(begin + j) * pk.k_stride + kh * D;
+        const uint16_t *v = pk.v + (size_t)(begin + j) * pk.v_stride + kh * D;
         float t = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) t = fmaf(q[i], bf16_f32(k[lane * N + i]), t);

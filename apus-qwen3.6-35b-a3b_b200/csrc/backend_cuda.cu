@@ -22,7 +22,9 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attn_decode.cuh"
 #include "attn_rows.cuh"
+#include "attn_view.cuh"
 #include "common.cuh"
 #include "decode_fused.cuh"
 #include "decode_stack.cuh"
@@ -128,6 +130,9 @@ struct Ctx {
     unsigned long long *d_df_timeline = nullptr;   /* [sm_count][DF_MARKS] */
     bool df_timeline_valid = false;
     int ds_absent = -1;
+    /* unfinished results of attention over the paged cache (attn_decode.cuh) */
+    float *d_attn_parts = nullptr;
+    int *d_attn_items = nullptr;
     size_t df_act_elems = 0, df_sa_elems = 0;
     int last_block_launches = 0;
     int last_block_path = 0;
@@ -248,6 +253,8 @@ static int ctx_init() {
     CU_OK(cudaMemset(c->d_df_sync, 0, 64));
     CU_OK(cudaMalloc(&c->d_df_timeline,
                      (size_t)c->sm_count * DF_MARKS * sizeof(unsigned long long)));
+    CU_OK(cudaMalloc(&c->d_attn_parts, ad_scratch_floats(c->sm_count) * sizeof(float)));
+    CU_OK(cudaMalloc(&c->d_attn_items, (size_t)c->sm_count * 2 * sizeof(int)));
     g_apus_use_pdl = env_long("APUS_CUDA_PDL", 1) != 0;
     g_pg_overlap = (int)env_long("APUS_CUDA_GEMM_OVERLAP", 1);
     g_pg_dynamic = (int)env_long("APUS_CUDA_GEMM_DYNAMIC", 3);
@@ -446,6 +453,8 @@ extern "C" void apus_cuda_disable(void) {
     if (c->d_ds_codes) cudaFree(c->d_ds_codes);
     if (c->d_ds_chains) cudaFree(c->d_ds_chains);
     if (c->d_df_timeline) cudaFree(c->d_df_timeline);
+    if (c->d_attn_parts) cudaFree(c->d_attn_parts);
+    if (c->d_attn_items) cudaFree(c->d_attn_items);
     if (c->d_df_act) cudaFree(c->d_df_act);
     if (c->d_df_sa) cudaFree(c->d_df_sa);
     if (c->d_router_logits) cudaFree(c->d_router_logits);
