@@ -64,6 +64,25 @@ static int kv_view(const ApusCudaKvCache *kv, const char *what, KvView *out) {
         g_ctx->launches++;                                                       \
     } while (0)
 
+/* all CTAs at the same time */
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_coop_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                 cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_apus_use_pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 static unsigned kv_apply_grid(const Ctx *c) {
     return (unsigned)c->sm_count * (2048 / KV_APPLY_THREADS);
 }
@@ -341,9 +360,8 @@ static int launch_decode(Ctx *c, const CUtensorMap &mk, const CUtensorMap &mv, D
     for (int row = 0; row < p.a.rows; row += AD_MAX_ROWS) {
         p.row0 = row;
         p.rows = p.a.rows - row < AD_MAX_ROWS ? p.a.rows - row : AD_MAX_ROWS;
-        LAUNCH_OK(launch_k(attn_decode_kernel<D, NH>, dim3(grid), dim3(AD_THREADS), smem, st, mk,
-                           mv, p));
-        LAUNCH_OK(launch_k(attn_join_kernel<D>, dim3(grid, p.a.group), dim3(D), 0, st, p, grid));
+        LAUNCH_OK(launch_coop_k(attn_decode_kernel<D, NH>, dim3(grid), dim3(AD_THREADS), smem, st,
+                                mk, mv, p));
     }
     return 0;
 }
@@ -365,6 +383,7 @@ extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKv
     p.status = kv->work;
     p.pages = c.pages;
     p.page_tokens = c.page_tokens;
+    p.page_tiles = c.page_tokens / AD_TILE;
     p.seqs = c.seqs;
     p.max_pages = c.max_pages;
     p.kv_heads = (int)kv->kv_heads;
@@ -380,8 +399,10 @@ extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKv
     Ordered ord(x, st);
     if (ord.rc) return 1;
     p.wait_status = x->d_status;
-    p.parts = x->d_attn_parts;
-    p.items = x->d_attn_items;
+    p.shared_parts = x->d_attn_parts;
+    p.parts = reinterpret_cast<float *>(x->d_attn_parts +
+                                        (size_t)x->sm_count * 2 * AD_SHARED_WORDS);
+    p.sync = x->d_attn_sync;
     const bool wide = p.a.group > 8;
     if (D == 64) return wide ? launch_decode<64, 16>(x, mk, mv, p, st)
                              : launch_decode<64, 8>(x, mk, mv, p, st);

@@ -19,8 +19,9 @@
  *                                                 accumulators as they lie, narrowed to BF16
  *
  * A piece that holds a sequence's tokens only in part leaves (max, sum, outputs) behind: those of
- * one SM are put together in shared memory, those of several SMs by attn_join_kernel, always in
- * the order of the line, so that a result does not depend on timing.
+ * one SM are put together in shared memory, those of several SMs by these SMs, each a share of
+ * the values, as they arrive (a cooperative launch: all CTAs run at the same time, and a wait
+ * has a limit); always in the same order, so that a result does not depend on timing.
  */
 #pragma once
 #include <cuda.h>
@@ -40,26 +41,35 @@ constexpr int AD_TILE = 16;                  /* tokens */
 constexpr int AD_MAX_ROWS = 1024;            /* of a launch */
 constexpr int AD_RING_BYTES = 24 << 10;      /* of a warp */
 constexpr int AD_MAX_CTAS = 256;
+constexpr int AD_SYNC_ROUND = 0, AD_SYNC_SEEN = 32, AD_SYNC_WORDS = 64;
 constexpr int AD_MAX_GROUP = 16;
 constexpr int AD_MAX_DIM = 256;
-/* one unfinished result: outputs, then max and sum of each head */
-constexpr int AD_PART_FLOATS = AD_MAX_GROUP * AD_MAX_DIM + 2 * AD_MAX_GROUP;
+/* one unfinished result: outputs, four floats between heads (the accumulators' lanes then
+ * write to 32 banks), then max and sum of each head */
+constexpr int AD_PAD = 4;
+constexpr int AD_PART_ML = AD_MAX_GROUP * (AD_MAX_DIM + AD_PAD);
+constexpr int AD_PART_FLOATS = AD_PART_ML + 2 * AD_MAX_GROUP;
 
 struct DecodeParams {
     AttnView a;
     const int32_t *table, *len, *seq;
     int32_t *status;                         /* the cache's */
     int *wait_status;                        /* the library's */
-    int pages, page_tokens, seqs, max_pages, kv_heads;
+    int pages, page_tokens, page_tiles, seqs, max_pages, kv_heads;
     int row0, rows;                          /* of this launch */
-    /* [gridDim][2] parts of this launch's CTAs: 0 began in an earlier CTA, 1 goes on in a later one;
-     * then one for each warp: what ends in it and began in an earlier one */
-    float *parts;
-    int *items;                              /* [gridDim][2] whose they are, -1: none */
+    uint2 *shared_parts;                     /* [gridDim][2]: began in an earlier CTA, or here */
+    float *parts;                            /* [gridDim][warps]: ends in the warp, began before it */
+    unsigned *sync;                          /* rounds so far, CTAs that have seen the number */
 };
 
-inline size_t ad_scratch_floats(int sms) {
-    return (size_t)sms * (2 + AD_WARPS) * AD_PART_FLOATS;
+/* a part as other SMs read it: every float beside the number of the round that wrote it, so that
+ * it is its own flag (no fence, no second look): (value, round) words, outputs and then a
+ * head's max and sum side by side */
+constexpr int AD_SHARED_ML = AD_MAX_GROUP * AD_MAX_DIM;
+constexpr int AD_SHARED_WORDS = AD_SHARED_ML + 2 * AD_MAX_GROUP;
+inline size_t ad_scratch_bytes(int sms) {
+    return (size_t)sms * (2 * AD_SHARED_WORDS * sizeof(uint2) +
+                          AD_WARPS * AD_PART_FLOATS * sizeof(float));
 }
 
 template <int D>
@@ -76,6 +86,9 @@ struct AdShared {
     float m[AD_WARPS][2][AD_MAX_GROUP], l[AD_WARPS][2][AD_MAX_GROUP];
     int item[AD_WARPS][2];
     long long scan[AD_WARPS];
+    float weight[2 * AD_WARPS][AD_MAX_GROUP], top[2 * AD_WARPS][AD_MAX_GROUP],
+        sum[2 * AD_WARPS][AD_MAX_GROUP];
+    int leads[2 * AD_WARPS], joint[2];
 };
 inline int ad_smem_bytes() { return AD_WARPS * AD_RING_BYTES + (int)sizeof(AdShared) + 1024; }
 
@@ -115,7 +128,12 @@ struct AdCursor {
         row = lo;
         tiles = (int)(s.start[row + 1] - s.start[row]);
         const long long in = at - s.start[row] * kv_heads;
-        head = tiles ? (int)(in / tiles) : 0;
+        head = 0;
+        if (tiles) {                         /* in / tiles, without a 64-bit division */
+            head = (int)((double)in / (double)tiles);
+            if ((long long)head * tiles > in) head--;
+            if ((long long)(head + 1) * tiles <= in) head++;
+        }
         tile = tiles ? (int)(in - (long long)head * tiles) : 0;
     }
     __device__ __forceinline__ void next_item(const AdShared &s, int rows, int kv_heads) {
@@ -129,10 +147,98 @@ struct AdCursor {
     }
 };
 
-/* o of one head, narrowed once: gate included */
-__device__ __forceinline__ uint16_t ad_out(const AttnView &a, long row, int at, float y) {
-    if (a.gate) y *= sigmoid_f32(bf16_f32(a.gate[row * a.gate_stride + at]));
-    return bf16_bits(y);
+/* o narrowed once, the gate included (its sigmoid to a few 2^-23: no step of a BF16 result) */
+__device__ __forceinline__ float ad_gate(float g) {
+    return __fdividef(1.0f, 1.0f + __expf(-g));
+}
+/* an 8 x 8 tile of 16-bit values, two to a lane, the other way round */
+__device__ __forceinline__ uint32_t ad_transpose(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void ad_store4(const AttnView &a, long row, int at, float4 y) {
+    if (a.gate) {
+        const uint2 g = *reinterpret_cast<const uint2 *>(a.gate + row * a.gate_stride + at);
+        y.x *= ad_gate(bf16lo(g.x));
+        y.y *= ad_gate(bf16hi(g.x));
+        y.z *= ad_gate(bf16lo(g.y));
+        y.w *= ad_gate(bf16hi(g.y));
+    }
+    *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + at) =
+        make_uint2(pack_bf16_rn(y.x, y.y), pack_bf16_rn(y.z, y.w));
+}
+
+/* an item, and whether a CTA's piece of the line holds all of it */
+struct AdItem {
+    int row, head;
+    long long begin, tiles;
+    bool before, after;
+    __device__ __forceinline__ AdItem(const AdShared &s, int item, int kv_heads, long long lo,
+                                      long long hi) {
+        row = item / kv_heads;
+        head = item - row * kv_heads;
+        tiles = s.start[row + 1] - s.start[row];
+        begin = s.start[row] * kv_heads + (long long)head * tiles;
+        before = begin < lo;
+        after = begin + tiles > hi;
+    }
+};
+/* (top, sum, acc) and another part's: both maxima may be of nothing */
+__device__ __forceinline__ void ad_merge(float &top, float &sum, float4 &acc, float pm, float ps,
+                                         float4 v) {
+    const float t = fmaxf(top, pm), base = t == -INFINITY ? 0.0f : t;
+    const float a = exp2_fast(top - base), b = exp2_fast(pm - base);
+    top = t;
+    sum = a * sum + b * ps;
+    acc.x = a * acc.x + b * v.x;
+    acc.y = a * acc.y + b * v.y;
+    acc.z = a * acc.z + b * v.z;
+    acc.w = a * acc.w + b * v.w;
+}
+/* four values of a head's sums as they leave */
+__device__ __forceinline__ void ad_finish4(const AttnView &a, long row, int head, int D, int c,
+                                           float4 acc, float top, float sum) {
+    const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+    acc.x *= inv;
+    acc.y *= inv;
+    acc.z *= inv;
+    acc.w *= inv;
+    ad_store4(a, row, head * D + c, acc);
+    if (c == 0 && a.lse)
+        a.lse[row * a.heads + head] = sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+}
+__device__ __forceinline__ void ad_put2(uint2 *at, float x, float y, unsigned round) {
+    asm volatile("st.relaxed.gpu.global.v4.u32 [%0], {%1, %2, %3, %2};" ::"l"(at),
+                 "r"(__float_as_uint(x)), "r"(round), "r"(__float_as_uint(y))
+                 : "memory");
+}
+__device__ __forceinline__ uint4 ad_look2(const uint2 *at) {
+    uint4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(at)
+                 : "memory");
+    return v;
+}
+/* four values and a head's max and sum of this round, for about a second at most */
+__device__ __forceinline__ bool ad_get(const uint2 *at, const uint2 *at_ml, unsigned round,
+                                       uint4 &a, uint4 &b, uint4 &ml) {
+    for (uint32_t i = 0; i < APUS_WAIT_LIMIT; i++) {
+        a = ad_look2(at);
+        b = ad_look2(at + 2);
+        ml = ad_look2(at_ml);
+        if (a.y == round && a.w == round && b.y == round && b.w == round && ml.y == round &&
+            ml.w == round)
+            return true;
+        if (i > 64) __nanosleep(64);
+    }
+    return false;
+}
+/* place / per (per > 0) */
+__device__ __forceinline__ int ad_piece_of(long long place, long long per) {
+    if (place < 0x40000000) return (int)((unsigned)place / (unsigned)min(per, 0x7fffffffLL));
+    return (int)(place / per);
 }
 
 template <int D, int NH>
@@ -154,6 +260,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
         mbar_fence_init();
     }
     pdl_enter();
+    /* this round's number: no word holds it yet */
+    const unsigned round = *reinterpret_cast<volatile unsigned *>(p.sync + AD_SYNC_ROUND) + 1;
 
     /* ---- the line: tiles before every row (each CTA for itself) ---- */
     {
@@ -193,8 +301,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
         if (tid < 2 * AD_WARPS) s.item[tid >> 1][tid & 1] = -1;
     }
     __syncthreads();
+    /* all of this CTA has the round's number; the CTA that is last in this makes the next one */
+    unsigned seen = 0;
+    if (tid == 0) seen = atomicInc(p.sync + AD_SYNC_SEEN, gridDim.x - 1);
     const long long total = s.start[p.rows] * p.kv_heads;
-    long long per = (total + gridDim.x - 1) / gridDim.x;
+    long long per = total < 0x40000000 ? ((unsigned)total + gridDim.x - 1) / gridDim.x
+                                       : (total + gridDim.x - 1) / gridDim.x;
     if (per < AD_WARPS) per = AD_WARPS;                   /* one tile to a warp */
     const long long lo = min(total, per * blockIdx.x), hi = min(total, lo + per);
     const long long from = lo + (hi - lo) * warp / AD_WARPS,
@@ -234,10 +346,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 page_row = ci.row;
                 page_base = ci.tile;
                 const int tile = page_base + lane;
-                page_lane = tile < ci.tiles
-                                ? p.table[(size_t)s.seq[ci.row] * p.max_pages +
-                                          (unsigned)(tile * AD_TILE) / (unsigned)p.page_tokens]
-                                : 0;
+                page_lane = tile < ci.tiles ? p.table[(size_t)s.seq[ci.row] * p.max_pages +
+                                                      (unsigned)tile / (unsigned)p.page_tiles]
+                                            : 0;
             }
             int page = __shfl_sync(0xffffffffu, page_lane, ci.tile - page_base);
             count = min(AD_TILE, s.len[ci.row] - ci.tile * AD_TILE);
@@ -247,7 +358,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 count = 0;
             }
             coord = (page * p.kv_heads + ci.head) * p.page_tokens +
-                    (int)((unsigned)(ci.tile * AD_TILE) % (unsigned)p.page_tokens);
+                    (int)((unsigned)ci.tile % (unsigned)p.page_tiles) * AD_TILE;
         }
         if (lane == 0) {
             s.valid[warp][st] = count;
@@ -286,7 +397,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 for (int j = 0; j < 4; j++) o[n][k][j] = 0.0f;
         }
     };
-    /* an unfinished result in fp32: [group][D] */
+    /* an unfinished result in fp32 */
     auto leave = [&](float *dst, int slot) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -296,7 +407,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 if (h < group)
 #pragma unroll
                     for (int k = 0; k < MT; k++)
-                        dst[h * D + k * 16 + (j >> 1) * 8 + g] = o[n][k][j];
+                        dst[h * (D + AD_PAD) + k * 16 + (j >> 1) * 8 + g] = o[n][k][j];
             }
             if (t4 == 0) {
                 s.m[warp][slot][n * 8 + g] = m[n];
@@ -304,8 +415,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             }
         }
     };
-    const size_t warp_part =
-        (size_t)(2 * gridDim.x + blockIdx.x * AD_WARPS + warp) * AD_PART_FLOATS;
+    const size_t warp_part = (size_t)(blockIdx.x * AD_WARPS + warp) * AD_PART_FLOATS;
     bool first = cc.tile > 0;              /* the item began before this piece */
     if (from < to) begin();
     while (alive && done < to) {
@@ -434,20 +544,32 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 if (p.a.lse && t4 == 0 && n * 8 + g < group)
                     p.a.lse[row * p.a.heads + h0 + n * 8 + g] =
                         l[n] > 0.0f ? (m[n] + log2f(l[n])) * LN2 : -INFINITY;
+                const float v0 = __shfl_sync(0xffffffffu, inv, t4 * 8),
+                            v1 = __shfl_sync(0xffffffffu, inv, t4 * 8 + 4);
+                /* the accumulators hold (value g; heads 2 t, 2 t + 1); memory wants (head g;
+                 * values 2 t, 2 t + 1): 8 x 8 transposes, of the gate on its way in */
+                const int at = (h0 + n * 8 + g) * D + t4 * 2;
+                const bool there = n * 8 + g < group;
+                uint32_t gt[2 * MT];
+                if (p.a.gate)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float v = __shfl_sync(0xffffffffu, inv, t4 * 8 + j * 4);
-                    const int h = n * 8 + t4 * 2 + j;
-                    if (h < group) {
+                    for (int k = 0; k < 2 * MT; k++)
+                        gt[k] = there ? __ldg(reinterpret_cast<const uint32_t *>(
+                                            p.a.gate + row * p.a.gate_stride + at + k * 8))
+                                      : 0u;
 #pragma unroll
-                        for (int k = 0; k < MT; k++)
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                const int at = (h0 + h) * D + k * 16 + i * 8 + g;
-                                p.a.out[row * p.a.out_stride + at] =
-                                    ad_out(p.a, row, at, o[n][k][i * 2 + j] * v);
-                            }
+                for (int k = 0; k < 2 * MT; k++) {
+                    float y0 = o[n][k >> 1][(k & 1) * 2] * v0,
+                          y1 = o[n][k >> 1][(k & 1) * 2 + 1] * v1;
+                    if (p.a.gate) {
+                        const uint32_t x = ad_transpose(gt[k]);
+                        y0 *= ad_gate(bf16lo(x));
+                        y1 *= ad_gate(bf16hi(x));
                     }
+                    const uint32_t y = ad_transpose(pack_bf16_rn(y0, y1));
+                    if (there)
+                        *reinterpret_cast<uint32_t *>(p.a.out + row * p.a.out_stride + at +
+                                                      k * 8) = y;
                 }
             }
         } else if (done == to) {                          /* in the ring, once all is through */
@@ -473,110 +595,136 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     __syncthreads();
 
     /* ---- the SM's unfinished results, put together in the order of the line ---- */
-    if (tid < 2) p.items[blockIdx.x * 2 + tid] = -1;
-    __syncthreads();
-    for (int e = 0; e < 2 * AD_WARPS;) {
+    constexpr int ENTRIES = 2 * AD_WARPS;
+    {                                                     /* the weight of an entry's head */
+        const int e = tid / AD_MAX_GROUP, h = tid % AD_MAX_GROUP;
         const int item = s.item[e >> 1][e & 1];
-        if (item < 0) {
-            e++;
-            continue;
-        }
-        int end = e + 1;                                  /* entries of the same item */
-        while (end < 2 * AD_WARPS && (s.item[end >> 1][end & 1] == item ||
-                                      s.item[end >> 1][end & 1] < 0))
-            end++;
-        const int r = item / p.kv_heads, kh = item - r * p.kv_heads;
-        const long long begin_at =
-            s.start[r] * p.kv_heads + (long long)kh * (s.start[r + 1] - s.start[r]);
-        const long long end_at = begin_at + (s.start[r + 1] - s.start[r]);
-        const bool before = begin_at < lo, after = end_at > hi;
-        const long row = p.row0 + r;
-        float *part = p.parts + (size_t)(blockIdx.x * 2 + (before ? 0 : 1)) * AD_PART_FLOATS;
-        for (int i = tid; i < group * D; i += AD_THREADS) {
-            const int h = i / D;
-            float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-            for (int j = e; j < end; j++)
-                if (s.item[j >> 1][j & 1] >= 0) top = fmaxf(top, s.m[j >> 1][j & 1][h]);
-            for (int j = e; j < end; j++) {
-                const int w = j >> 1;
-                if (s.item[w][j & 1] < 0 || s.m[w][j & 1][h] == -INFINITY) continue;
-                const float f = exp2_fast(s.m[w][j & 1][h] - top);
-                const float *src =
-                    j & 1 ? reinterpret_cast<float *>(ring0) + w * (AD_RING_BYTES / 4)
-                          : p.parts + (size_t)(2 * gridDim.x + blockIdx.x * AD_WARPS + w) *
-                                          AD_PART_FLOATS;
-                sum = fmaf(f, s.l[w][j & 1][h], sum);
-                acc = fmaf(f, src[i], acc);
-            }
-            if (before || after) {
-                part[i] = acc;
-                if (i % D == 0) {
-                    part[AD_MAX_GROUP * AD_MAX_DIM + h] = top;
-                    part[AD_MAX_GROUP * AD_MAX_DIM + AD_MAX_GROUP + h] = sum;
+        float top = -INFINITY, sum = 0.0f;
+        bool leads = item >= 0;
+        if (item >= 0 && h < group) {
+#pragma unroll
+            for (int j = 0; j < ENTRIES; j++)
+                if (s.item[j >> 1][j & 1] == item) top = fmaxf(top, s.m[j >> 1][j & 1][h]);
+            if (top == -INFINITY) top = 0.0f;             /* nothing counted: weights of 0 */
+#pragma unroll
+            for (int j = 0; j < ENTRIES; j++)
+                if (s.item[j >> 1][j & 1] == item) {
+                    sum = fmaf(exp2_fast(s.m[j >> 1][j & 1][h] - top), s.l[j >> 1][j & 1][h], sum);
+                    if (j < e) leads = false;
                 }
-            } else {
-                const int at = kh * group * D + i;
-                p.a.out[row * p.a.out_stride + at] =
-                    ad_out(p.a, row, at, sum > 0.0f ? __fdividef(acc, sum) : 0.0f);
-                if (p.a.lse && i % D == 0)
-                    p.a.lse[row * p.a.heads + kh * group + h] =
-                        sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
-            }
+            s.weight[e][h] = exp2_fast(s.m[e >> 1][e & 1][h] - top);
+            s.top[e][h] = top;
+            s.sum[e][h] = sum;
         }
-        if (tid == 0 && (before || after)) p.items[blockIdx.x * 2 + (before ? 0 : 1)] = item;
-        e = end;
+        if (h == 0) s.leads[e] = leads;
     }
-}
+    __syncthreads();
+    constexpr int HEAD4 = D / 4;                          /* pieces of 16 bytes of a head */
+    const int per_item = group * HEAD4;
+    int items = 0;
+#pragma unroll
+    for (int e = 0; e < ENTRIES; e++) items += s.leads[e];
+#pragma unroll 1
+    for (int x = tid; x < items * per_item; x += AD_THREADS) {
+        int e = -1, nth = x / per_item;
+        const int in = x - nth * per_item, h = in / HEAD4, c = (in - h * HEAD4) * 4;
+        do
+            nth -= s.leads[++e];
+        while (nth >= 0);
+        const int item = s.item[e >> 1][e & 1];
+        float4 v[ENTRIES];
+        float f[ENTRIES];
+#pragma unroll
+        for (int j = 0; j < ENTRIES; j++) {
+            const int w = j >> 1;
+            const bool of = s.item[w][j & 1] == item;
+            const int from_at = h * (D + AD_PAD) + c;
+            f[j] = of ? s.weight[j][h] : 0.0f;
+            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (of)
+                v[j] = j & 1 ? *reinterpret_cast<const float4 *>(
+                                   ring0 + w * AD_RING_BYTES + from_at * 4)
+                             : *reinterpret_cast<const float4 *>(
+                                   p.parts + (size_t)(blockIdx.x * AD_WARPS + w) * AD_PART_FLOATS + from_at);
+        }
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < ENTRIES; j++) {
+            acc.x = fmaf(f[j], v[j].x, acc.x);
+            acc.y = fmaf(f[j], v[j].y, acc.y);
+            acc.z = fmaf(f[j], v[j].z, acc.z);
+            acc.w = fmaf(f[j], v[j].w, acc.w);
+        }
+        const AdItem it(s, item, p.kv_heads, lo, hi);
+        const float top = s.top[e][h], sum = s.sum[e][h];
+        if (it.before || it.after) {
+            uint2 *part = p.shared_parts + (size_t)(blockIdx.x * 2 + !it.before) * AD_SHARED_WORDS;
+            ad_put2(part + h * D + c, acc.x, acc.y, round);
+            ad_put2(part + h * D + c + 2, acc.z, acc.w, round);
+            if (c == 0) ad_put2(part + AD_SHARED_ML + 2 * h, top, sum, round);
+        } else {
+            ad_finish4(p.a, p.row0 + it.row, it.head * group + h, D, c, acc, top, sum);
+        }
+    }
 
-/* An item that several SMs hold parts of begins in one of them: a CTA for each SM and head looks
- * whether one begins there, and adds up its parts in order. */
-template <int D>
-__global__ void __launch_bounds__(D) attn_join_kernel(const __grid_constant__ DecodeParams p,
-                                                      int ctas) {
-    pdl_enter();
-    const int c = blockIdx.x, h = blockIdx.y, i = threadIdx.x, group = p.a.group;
-    const int item = p.items[c * 2 + 1];
-    if (item < 0) return;
-    __shared__ int s_end;
-    __shared__ float weight[AD_MAX_CTAS], sums[AD_MAX_CTAS];
-    if (i == 0) s_end = ctas;
+    /* ---- items that several SMs hold parts of ---- */
+    if (tid < 2) s.joint[tid] = -1;
     __syncthreads();
-    for (int e = c + 1 + i; e < ctas; e += D)
-        if (p.items[e * 2] != item) {
-            atomicMin(&s_end, e);
-            break;
+    if (tid < ENTRIES && s.leads[tid]) {
+        const int item = s.item[tid >> 1][tid & 1];
+        const AdItem it(s, item, p.kv_heads, lo, hi);
+        if (it.before || it.after) s.joint[!it.before] = item;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int j = 0; j < 2; j++) {
+        const int item = s.joint[j];
+        if (item < 0) continue;
+        const AdItem it(s, item, p.kv_heads, lo, hi);
+        const int c0 = ad_piece_of(it.begin, per),
+                  n = ad_piece_of(it.begin + it.tiles - 1, per) - c0 + 1;
+        /* every SM that holds a part adds up a share of the pieces: a few lanes to a piece, each
+         * some of the parts, then the lanes by shuffles */
+        const int share = (per_item + n - 1) / n, first_piece = share * ((int)blockIdx.x - c0);
+        const int pieces = min(share, per_item - first_piece);
+        if (pieces <= 0) continue;
+        int lanes = 32;
+        while (lanes > 1 && lanes * pieces > AD_THREADS) lanes >>= 1;
+        const int sub = tid & (lanes - 1);
+#pragma unroll 1
+        for (int x0 = tid / lanes; x0 - tid / lanes < pieces; x0 += AD_THREADS / lanes) {
+            const bool real = x0 < pieces;
+            const int in = first_piece + (real ? x0 : 0), h = in / HEAD4, c = (in - h * HEAD4) * 4;
+            float top = -INFINITY, sum = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int e = sub; e < n; e += lanes) {
+                const uint2 *part =
+                    p.shared_parts + (size_t)((c0 + e) * 2 + (e == 0)) * AD_SHARED_WORDS;
+                uint4 a, b, ml;
+                if (!ad_get(part + h * D + c, part + AD_SHARED_ML + 2 * h, round, a, b, ml)) {
+                    set_status(p.wait_status, ST_SCHED_TIMEOUT);
+                    break;
+                }
+                ad_merge(top, sum, acc, __uint_as_float(ml.x), __uint_as_float(ml.z),
+                         make_float4(__uint_as_float(a.x), __uint_as_float(a.z),
+                                     __uint_as_float(b.x), __uint_as_float(b.z)));
+            }
+            for (int o = 1; o < lanes; o <<= 1) {
+                float4 v;
+                const float pm = __shfl_xor_sync(0xffffffffu, top, o),
+                            ps = __shfl_xor_sync(0xffffffffu, sum, o);
+                v.x = __shfl_xor_sync(0xffffffffu, acc.x, o);
+                v.y = __shfl_xor_sync(0xffffffffu, acc.y, o);
+                v.z = __shfl_xor_sync(0xffffffffu, acc.z, o);
+                v.w = __shfl_xor_sync(0xffffffffu, acc.w, o);
+                ad_merge(top, sum, acc, pm, ps, v);
+            }
+            if (real && sub == 0)
+                ad_finish4(p.a, p.row0 + it.row, it.head * group + h, D, c, acc, top, sum);
         }
-    __syncthreads();
-    const int end = s_end;
-    auto part = [&](int e) {
-        return p.parts + (size_t)(e * 2 + (e == c ? 1 : 0)) * AD_PART_FLOATS;
-    };
-    constexpr int ML = AD_MAX_GROUP * AD_MAX_DIM;
-    const int parts = end - c;
-    for (int e = i; e < parts; e += D) {
-        weight[e] = part(c + e)[ML + h];
-        sums[e] = part(c + e)[ML + AD_MAX_GROUP + h];
     }
-    __syncthreads();
-    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (int e = 0; e < parts; e++) top = fmaxf(top, weight[e]);
-    if (top == -INFINITY) top = 0.0f;                     /* nothing counted: weights of 0 */
-    __syncthreads();
-    for (int e = i; e < parts; e += D) weight[e] = exp2_fast(weight[e] - top);
-    __syncthreads();
-#pragma unroll 16
-    for (int e = 0; e < parts; e++) {
-        sum = fmaf(weight[e], sums[e], sum);
-        acc = fmaf(weight[e], part(c + e)[h * D + i], acc);
-    }
-    const int r = item / p.kv_heads, kh = item - r * p.kv_heads;
-    const long row = p.row0 + r;
-    const int at = (kh * group + h) * D + i;
-    p.a.out[row * p.a.out_stride + at] =
-        ad_out(p.a, row, at, sum > 0.0f ? __fdividef(acc, sum) : 0.0f);
-    if (p.a.lse && i == 0)
-        p.a.lse[row * p.a.heads + kh * group + h] =
-            sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+    if (tid == 0 && seen == gridDim.x - 1) atomicAdd(p.sync + AD_SYNC_ROUND, 1u);
 }
 
 }  // namespace apus

@@ -131,8 +131,8 @@ struct Ctx {
     bool df_timeline_valid = false;
     int ds_absent = -1;
     /* unfinished results of attention over the paged cache (attn_decode.cuh) */
-    float *d_attn_parts = nullptr;
-    int *d_attn_items = nullptr;
+    uint2 *d_attn_parts = nullptr;
+    unsigned *d_attn_sync = nullptr;
     size_t df_act_elems = 0, df_sa_elems = 0;
     int last_block_launches = 0;
     int last_block_path = 0;
@@ -253,8 +253,10 @@ static int ctx_init() {
     CU_OK(cudaMemset(c->d_df_sync, 0, 64));
     CU_OK(cudaMalloc(&c->d_df_timeline,
                      (size_t)c->sm_count * DF_MARKS * sizeof(unsigned long long)));
-    CU_OK(cudaMalloc(&c->d_attn_parts, ad_scratch_floats(c->sm_count) * sizeof(float)));
-    CU_OK(cudaMalloc(&c->d_attn_items, (size_t)c->sm_count * 2 * sizeof(int)));
+    CU_OK(cudaMalloc(&c->d_attn_parts, ad_scratch_bytes(c->sm_count)));
+    CU_OK(cudaMemset(c->d_attn_parts, 0, ad_scratch_bytes(c->sm_count)));
+    CU_OK(cudaMalloc(&c->d_attn_sync, AD_SYNC_WORDS * sizeof(unsigned)));
+    CU_OK(cudaMemset(c->d_attn_sync, 0, AD_SYNC_WORDS * sizeof(unsigned)));
     g_apus_use_pdl = env_long("APUS_CUDA_PDL", 1) != 0;
     g_pg_overlap = (int)env_long("APUS_CUDA_GEMM_OVERLAP", 1);
     g_pg_dynamic = (int)env_long("APUS_CUDA_GEMM_DYNAMIC", 3);
@@ -454,7 +456,7 @@ extern "C" void apus_cuda_disable(void) {
     if (c->d_ds_chains) cudaFree(c->d_ds_chains);
     if (c->d_df_timeline) cudaFree(c->d_df_timeline);
     if (c->d_attn_parts) cudaFree(c->d_attn_parts);
-    if (c->d_attn_items) cudaFree(c->d_attn_items);
+    if (c->d_attn_sync) cudaFree(c->d_attn_sync);
     if (c->d_df_act) cudaFree(c->d_df_act);
     if (c->d_df_sa) cudaFree(c->d_df_sa);
     if (c->d_router_logits) cudaFree(c->d_router_logits);
