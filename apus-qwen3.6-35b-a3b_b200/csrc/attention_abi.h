@@ -169,7 +169,7 @@ extern "C" int apus_cuda_kv_copy_dev(const ApusCudaKvCache *kv, const int32_t *d
 /* a tensor of rows: its stride, or 0 where it is none that the kernels can read */
 static long row_stride(const void *p, size_t stride, size_t heads, size_t head_dim) {
     const size_t s = stride ? stride : heads * head_dim;
-    if (!p || !aligned16(p) || s % 8 || s < heads * head_dim || s > ((size_t)1 << 40)) return 0;
+    if (!p || !aligned16(p) || s % 8 || s < heads * head_dim || s > ((size_t)1 << 32)) return 0;
     return (long)s;
 }
 
@@ -292,45 +292,95 @@ static int attn_view(const ApusCudaAttn *a, const char *what, AttnView *out) {
     return 0;
 }
 
-static int launch_rows(const AttnView &a, size_t D, const AttnPacked &pk, cudaStream_t st) {
-    const dim3 grid((unsigned)(((size_t)a.rows * a.heads + 7) / 8));
-    if (D == 64) LAUNCH_OK(launch_k(attn_rows_kernel<64>, grid, dim3(256), 0, st, a, pk));
-    else if (D == 128) LAUNCH_OK(launch_k(attn_rows_kernel<128>, grid, dim3(256), 0, st, a, pk));
-    else LAUNCH_OK(launch_k(attn_rows_kernel<256>, grid, dim3(256), 0, st, a, pk));
+/* rows x heads x head_dim values as {64, heads, rows, head_dim / 64} or {64, rows, heads, ...}:
+ * boxes of one 128-byte swizzle row by `heads` and `rows` */
+static int attn_map(CUtensorMap *m, const uint16_t *base, size_t rows, size_t stride, size_t heads,
+                    size_t D, bool heads_first, int box_heads, int box_rows) {
+    PFN_encodeTiled_local enc = tensor_map_encoder();
+    if (!enc) return fail("%s", prefill_last_error());
+    const int h = heads_first ? 1 : 2, r = heads_first ? 2 : 1;
+    cuuint64_t dims[4] = {64, 0, 0, (cuuint64_t)(D / 64)}, strides[3] = {0, 0, 128};
+    cuuint32_t box[4] = {64, 0, 0, 1}, estr[4] = {1, 1, 1, 1};
+    dims[h] = heads;
+    dims[r] = rows;
+    strides[h - 1] = D * 2;
+    strides[r - 1] = stride * 2;
+    box[h] = (cuuint32_t)box_heads;
+    box[r] = (cuuint32_t)box_rows;
+    CUresult e = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t *>(base), dims,
+                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? 0
+                             : fail("attn_prompt_dev: cuTensorMapEncodeTiled failed (%d)", (int)e);
+}
+
+template <int D>
+static int launch_prompt(Ctx *c, const PromptParams &p, const ApusCudaAttnKeys *keys,
+                         long k_stride, long v_stride, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    /* no key at all: nothing is loaded, any address does */
+    const uint16_t *k = keys->rows ? keys->k : p.a.q, *v = keys->rows ? keys->v : p.a.q;
+    const size_t rows = keys->rows ? keys->rows : 1;
+    if (!keys->rows) k_stride = v_stride = (long)p.kv_heads * D;
+    if (attn_map(&mq, p.a.q, p.a.rows, p.a.q_stride, p.a.heads, D, true, p.a.group,
+                 p.tile_tokens) ||
+        attn_map(&mk, k, rows, k_stride, p.kv_heads, D, false, 1, AP_ROWS) ||
+        attn_map(&mv, v, rows, v_stride, p.kv_heads, D, false, 1, ApShape<D>::V_ROWS))
+        return 1;
+    constexpr int smem = ap_smem_bytes<D>();
+    static bool set = false;
+    if (!set) {
+        CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        set = true;
+    }
+    const int grid = p.items < c->sm_count ? p.items : c->sm_count;
+    LAUNCH_OK(launch_k(attn_prompt_kernel<D>, dim3(grid), dim3(AP_THREADS), smem, st, mq, mk, mv,
+                       p));
     return 0;
 }
 
 extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *keys,
                                          void *stream) {
     if (!a || !keys) return fail("attn_prompt_dev: bad args");
-    AttnView v;
-    if (attn_view(a, "attn_prompt_dev", &v)) return 1;
+    PromptParams p = {};
+    if (attn_view(a, "attn_prompt_dev", &p.a)) return 1;
     if (keys->rows > (1u << 30) || keys->seqs > (1u << 24))
         return fail("attn_prompt_dev: too many keys or sequences");
     if (!a->rows || !keys->seqs) return 0;
     if (!keys->cu_q || !keys->cu_k) return fail("attn_prompt_dev: bad args");
-    AttnPacked pk = {};
-    pk.k = keys->k;
-    pk.v = keys->v;
-    pk.cu_q = keys->cu_q;
-    pk.cu_k = keys->cu_k;
-    pk.rows = (int)keys->rows;
-    pk.seqs = (int)keys->seqs;
-    pk.causal = keys->causal != 0;
+    long k_stride = 0, v_stride = 0;
     if (keys->rows) {
-        pk.k_stride = row_stride(keys->k, keys->k_stride, a->kv_heads, a->head_dim);
-        pk.v_stride = row_stride(keys->v, keys->v_stride, a->kv_heads, a->head_dim);
-        if (!pk.k_stride || !pk.v_stride)
+        k_stride = row_stride(keys->k, keys->k_stride, a->kv_heads, a->head_dim);
+        v_stride = row_stride(keys->v, keys->v_stride, a->kv_heads, a->head_dim);
+        if (!k_stride || !v_stride)
             return fail("attn_prompt_dev: k or v is missing, or its address or stride is not a "
                         "multiple of 16 bytes or less than a row");
     }
+    p.cu_q = keys->cu_q;
+    p.cu_k = keys->cu_k;
+    p.k_rows = (int)keys->rows;
+    p.seqs = (int)keys->seqs;
+    p.causal = keys->causal != 0;
+    p.kv_heads = (int)a->kv_heads;
+    p.tile_tokens = AP_ROWS / p.a.group;
+    const size_t slots = a->rows / p.tile_tokens + keys->seqs;
+    if (slots * a->kv_heads > (1u << 30)) return fail("attn_prompt_dev: too many rows");
+    p.slots = (int)slots;
+    p.items = (int)(slots * a->kv_heads);
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
-    DeviceGuard dev(g_ctx->device);
+    Ctx *c = g_ctx;
+    DeviceGuard dev(c->device);
     cudaStream_t st = (cudaStream_t)stream;
-    Ordered ord(g_ctx, st);
+    Ordered ord(c, st);
     if (ord.rc) return 1;
-    return launch_rows(v, a->head_dim, pk, st);
+    p.sched = c->d_attn_sync + AD_SYNC_WORDS;
+    p.status = c->d_status;
+    if (a->head_dim == 64) return launch_prompt<64>(c, p, keys, k_stride, v_stride, st);
+    if (a->head_dim == 128) return launch_prompt<128>(c, p, keys, k_stride, v_stride, st);
+    return launch_prompt<256>(c, p, keys, k_stride, v_stride, st);
 }
 
 /* rows of head_dim values, 16 tokens of 64 values at a time, 128B swizzle */

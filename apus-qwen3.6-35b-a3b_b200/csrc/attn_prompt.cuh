@@ -1,0 +1,554 @@
+/*
+ * attn_prompt.cuh — attention of packed prompts on the 5th-generation tensor cores.
+ *
+ *   S = Q K^T,  p = exp2(scale log2(e) (S - m)) over the keys that a row sees,
+ *   O = P V / sum(p) * sigmoid(gate),  lse = log sum exp(scale S)
+ *
+ * One pass over the keys with a running maximum and sum.  The heads of a key head are rows: a
+ * tile of 128 rows is 128 / group tokens times the group's heads, so that short prompts fill it,
+ * every key is fetched once for all its heads, and the causal edge costs few masked scores.
+ *
+ * One persistent CTA per SM takes such tiles from a counter (the last tiles of each sequence
+ * first: they see the most keys).  Ten warps:
+ *   warp 0     finds the tile's sequence, loads Q (64 KB at head_dim 256) and a ring of 32 KB pieces of K and V
+ *   warp 1     issues tcgen05.mma: S(j+1) before O += P(j) V(j), so that the tensor cores work
+ *              while the softmax of a tile runs
+ *   warps 2-9  softmax: two warps to each quarter of the rows, each half of the 128 scores of a
+ *              row; outputs at the end
+ * S is double-buffered in tensor memory (2 x 128 columns), O takes head_dim columns.  P stays
+ * there as well: narrowed to BF16 it overwrites its own scores and is the MMA's A operand, so that
+ * shared memory carries Q, K and V only.  (K and Q are K-major; V's rows are its K dimension: the
+ * MN-major form of the same 128B-swizzled tile.)
+ *
+ * The maximum that a row's weights are taken against moves only when a score is 2^8 above it: any
+ * reference within the range of fp32 and BF16 gives the same quotient, and O in tensor memory
+ * is then hardly ever scaled again (that takes its 256 columns through registers).
+ *
+ * Bound at head_dim 256 and long prompts: the MMAs, 2048 cycles for 128 keys, beside 1024 of
+ * exponentials (16 a cycle and SM) on other units; at 128 and 64 the exponentials (1024
+ * against 1024 and 512).
+ */
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attn_decode.cuh"
+#include "attn_view.cuh"
+#include "common.cuh"
+#include "prefill_gemm.cuh"
+
+namespace apus {
+
+constexpr int AP_ROWS = 128;                 /* rows of a tile, keys of a step */
+constexpr int AP_SOFT_WARPS = 8;
+constexpr int AP_THREADS = 64 + AP_SOFT_WARPS * 32;
+constexpr int AP_TMEM_COLS = 512;
+constexpr int AP_TMEM_O = 256;               /* scores in columns 0..255 */
+constexpr int AP_ITEMS = 2;
+
+template <int D>
+struct ApShape {
+    static constexpr int BLOCKS = D / 64;                 /* of 64 values: a swizzle row */
+    static constexpr int Q_BYTES = AP_ROWS * D * 2;
+    static constexpr int UNITS = D == 256 ? 2 : 1;        /* pieces of a tile of K or of V */
+    static constexpr int UNIT_BYTES = AP_ROWS * D * 2 / UNITS;
+    static constexpr int V_ROWS = AP_ROWS / UNITS;        /* keys of a piece of V (all values) */
+    static constexpr int K_BLOCKS = BLOCKS / UNITS;       /* blocks of a piece of K (all keys) */
+    static constexpr int STAGES = D == 256 ? 5 : D == 128 ? 6 : 8;
+};
+
+struct PromptParams {
+    AttnView a;
+    const int32_t *cu_q, *cu_k;
+    int k_rows, seqs, causal, kv_heads;
+    int tile_tokens;                         /* 128 / group */
+    int slots, items;                        /* tiles that there may be, times key heads */
+    unsigned *sched;                         /* next item; [32]: CTAs that are through */
+    int *status;
+};
+
+struct ApItem {
+    int token, tokens;                       /* first row of q; tokens of the tile, -1: the end */
+    int head, tiles;                         /* key head, steps of 128 keys */
+    int key, keys;                           /* first row of k; keys that the last token sees */
+    int sees;                                /* keys that the first token sees */
+};
+struct ApShared {
+    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done, o_free;
+    uint64_t item_full[AP_ITEMS], item_empty[AP_ITEMS], pair[4];
+    ApItem item[AP_ITEMS];
+    uint32_t tmem;
+    int abort_flag;
+    uint16_t top[2][2][AP_ROWS];             /* a step's maxima, BF16: a reference needs no more */
+    float sum[2][AP_ROWS];
+};
+template <int D>
+constexpr int ap_smem_bytes() {
+    return ApShape<D>::Q_BYTES + ApShape<D>::STAGES * ApShape<D>::UNIT_BYTES +
+           (int)sizeof(ApShared);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                            int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::"
+        "complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+/* D[tmem] (+)= A[tmem] * B[smem] */
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                             uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, "
+        "%31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+/* B whose N dimension is contiguous (V: keys are K): 64 values x 8 keys to a swizzle atom of
+ * 1024 bytes, the next 8 keys SBO behind it, the next 64 values LBO */
+__device__ __forceinline__ uint64_t ap_desc_mn(uint32_t saddr, uint32_t block_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3ffffu) >> 4);
+    d |= (uint64_t)(block_bytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+constexpr uint32_t AP_B_MN = 1u << 16;       /* instruction descriptor: B is MN-major */
+
+/* The tile of an index, by a whole warp.  Sequence i's tiles have the slots from
+ * cu_q[i] / tile_tokens + i on: one more than it needs, at most, and no sums over sequences. */
+__device__ __forceinline__ ApItem ap_find(const PromptParams &p, int index) {
+    const int lane = threadIdx.x & 31, T = p.tile_tokens;
+    const int slot = p.slots - 1 - index / p.kv_heads;
+    auto base = [&](int i) { return __ldg(p.cu_q + i) / T + i; };
+    int lo = 0, hi = p.seqs;
+    while (hi - lo > 1) {                    /* the last sequence that starts at or before it */
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, at < hi && base(at) <= slot);
+        const int n = m ? 32 - __clz(m) : 1;
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    ApItem t;
+    const int q0 = min(max(__ldg(p.cu_q + lo), 0), p.a.rows),
+              q1 = min(max(__ldg(p.cu_q + lo + 1), q0), p.a.rows);
+    const int k0 = min(max(__ldg(p.cu_k + lo), 0), p.k_rows),
+              k1 = min(max(__ldg(p.cu_k + lo + 1), k0), p.k_rows);
+    const long first = (long)(slot - base(lo)) * T;       /* of the sequence's rows */
+    t.token = q0 + (int)first;
+    t.tokens = first < 0 || first >= q1 - q0 ? 0 : min(T, q1 - q0 - (int)first);
+    t.head = index % p.kv_heads;
+    t.key = k0;
+    t.keys = t.sees = k1 - k0;
+    if (p.causal) {
+        t.sees = k1 - k0 - (q1 - q0) + (int)first + 1;
+        t.keys = max(0, t.sees + t.tokens - 1);
+    }
+    t.tiles = (t.keys + AP_ROWS - 1) / AP_ROWS;
+    return t;
+}
+
+template <int D>
+__global__ void __launch_bounds__(AP_THREADS, 1)
+attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
+                   const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v,
+                   const __grid_constant__ PromptParams p) {
+    using S = ApShape<D>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ __align__(1024) unsigned char ap_smem[];
+    unsigned char *q_smem = ap_smem, *ring = ap_smem + S::Q_BYTES;
+    ApShared &s = *reinterpret_cast<ApShared *>(ring + STAGES * S::UNIT_BYTES);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(ap_smem) & 1023) {          /* swizzled tiles: the same answer in all threads */
+        if (tid == 0) set_status(p.status, ST_BAD_INDEX);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(&s.kv_full[i], 1);
+            mbar_init(&s.kv_empty[i], 1);
+        }
+        mbar_init(&s.q_full, 1);
+        mbar_init(&s.q_empty, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.p_full[i], AP_SOFT_WARPS);
+        }
+        mbar_init(&s.pv_done, 1);
+        mbar_init(&s.o_free, AP_SOFT_WARPS);
+        for (int i = 0; i < AP_ITEMS; i++) {
+            mbar_init(&s.item_full[i], 1);
+            mbar_init(&s.item_empty[i], 1 + AP_SOFT_WARPS);
+        }
+        for (int i = 0; i < 4; i++) mbar_init(&s.pair[i], 2);
+        s.abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&s.tmem, AP_TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    volatile int *abort_flag = &s.abort_flag;
+    pdl_enter();
+
+    /* the next tile, for all roles but the one that finds it */
+    auto next_item = [&](int n, ApItem &t) -> bool {
+        const int i = n % AP_ITEMS;
+        if (!pg_wait(&s.item_full[i], (uint32_t)(n / AP_ITEMS) & 1u, abort_flag, p.status,
+                     ST_SCHED_TIMEOUT))
+            return false;
+        t = s.item[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.item_empty[i]);
+        return t.tokens >= 0;
+    };
+
+    if (warp == 0) {
+        /* ---------------- tiles and loads ---------------- */
+        uint32_t unit = 0;
+        int full = 0;                        /* tiles that see keys, so far */
+        int index = blockIdx.x;
+        bool alive = true;
+        auto load = [&](bool keys, const ApItem &t, int j) {
+            for (int u = 0; u < S::UNITS && alive; u++, unit++) {
+                const int st = (int)(unit % STAGES);
+                if (!pg_wait(&s.kv_empty[st], ((unit / STAGES) & 1u) ^ 1u, abort_flag, p.status,
+                             ST_MBAR_TIMEOUT)) {
+                    alive = false;
+                    return;
+                }
+                const uint32_t dst = smem_u32(ring + st * S::UNIT_BYTES);
+                mbar_expect_tx(&s.kv_full[st], S::UNIT_BYTES);
+                if (keys) {
+#pragma unroll
+                    for (int b = 0; b < S::K_BLOCKS; b++)
+                        tma_load_4d(dst + b * AP_ROWS * 128, &map_k, 0, t.key + j * AP_ROWS,
+                                    t.head, u * S::K_BLOCKS + b, &s.kv_full[st]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < S::BLOCKS; b++)
+                        tma_load_4d(dst + b * S::V_ROWS * 128, &map_v, 0,
+                                    t.key + j * AP_ROWS + u * S::V_ROWS, t.head, b,
+                                    &s.kv_full[st]);
+                }
+            }
+        };
+        for (int n = 0; alive; n++) {
+            ApItem t;
+            t.tokens = -1;
+            while (index < p.items) {
+                t = ap_find(p, index);
+                if (t.tokens > 0) break;
+                t.tokens = -1;
+                index = p.items > (int)gridDim.x
+                            ? __shfl_sync(0xffffffffu,
+                                          lane == 0 ? (int)(gridDim.x + atomicAdd(p.sched, 1u)) : 0,
+                                          0)
+                            : p.items;
+            }
+            const int i = n % AP_ITEMS;
+            if (!pg_wait_warp(&s.item_empty[i], ((uint32_t)(n / AP_ITEMS) & 1u) ^ 1u, abort_flag,
+                              p.status, ST_SCHED_TIMEOUT))
+                break;
+            if (lane == 0) {
+                s.item[i] = t;
+                mbar_arrive(&s.item_full[i]);
+            }
+            __syncwarp();
+            if (t.tokens < 0) break;
+            if (lane == 0 && t.tiles > 0) {
+                if (!pg_wait(&s.q_empty, ((uint32_t)full & 1u) ^ 1u, abort_flag, p.status,
+                             ST_MBAR_TIMEOUT)) {
+                    alive = false;
+                } else {
+                    const int rows = p.a.group * p.tile_tokens;
+                    mbar_expect_tx(&s.q_full, (uint32_t)(S::BLOCKS * rows * 128));
+#pragma unroll
+                    for (int b = 0; b < S::BLOCKS; b++)
+                        tma_load_4d(smem_u32(q_smem + b * AP_ROWS * 128), &map_q, 0,
+                                    t.head * p.a.group, t.token, b, &s.q_full);
+                    load(true, t, 0);
+                    for (int j = 0; j < t.tiles && alive; j++) {
+                        if (j + 1 < t.tiles) load(true, t, j + 1);
+                        load(false, t, j);
+                    }
+                }
+            }
+            if (t.tiles > 0) full++;
+            index = p.items;
+            if (p.items > (int)gridDim.x) {
+                if (lane == 0) index = (int)(gridDim.x + atomicAdd(p.sched, 1u));
+                index = __shfl_sync(0xffffffffu, index, 0);
+            }
+            alive = __all_sync(0xffffffffu, alive);
+        }
+        /* the last CTA that asks no more sets the counters back */
+        if (lane == 0 && p.items > (int)gridDim.x) {
+            __threadfence();
+            if (atomicInc(p.sched + 32, gridDim.x - 1) == gridDim.x - 1) atomicExch(p.sched, 0u);
+        }
+    } else if (warp == 1) {
+        /* ---------------- MMA issuer ---------------- */
+        uint32_t unit = 0, scores = 0, sums = 0;
+        int full = 0;
+        bool alive = true;
+        const uint64_t q_desc = umma_smem_desc(smem_u32(q_smem));
+        const uint32_t ring_addr = smem_u32(ring);
+        ApItem t = {};
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            alive = alive && pg_wait_warp(bar, parity & 1u, abort_flag, p.status, ST_TMEM_TIMEOUT);
+            tc_fence_after();
+            return alive;
+        };
+        auto score = [&](int j) {
+            const uint32_t d = tmem + (scores & 1u) * AP_ROWS;
+            /* no more columns than there are keys (what lies behind them is masked) */
+            const int cols = min(AP_ROWS, ((t.keys - j * AP_ROWS) + 15) & ~15);
+            const uint32_t idesc = umma_idesc(cols);
+            for (int u = 0; u < S::UNITS; u++, unit++) {
+                const int st = (int)(unit % STAGES);
+                if (!wait(&s.kv_full[st], unit / STAGES)) return;
+                const uint64_t k_desc = umma_smem_desc(ring_addr + st * S::UNIT_BYTES);
+                if (pg_elect()) {
+#pragma unroll
+                    for (int b = 0; b < S::K_BLOCKS; b++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            umma_bf16(d,
+                                      q_desc + (uint64_t)((u * S::K_BLOCKS + b) * (AP_ROWS * 128 / 16) +
+                                                          2 * k),
+                                      k_desc + (uint64_t)(b * (AP_ROWS * 128 / 16) + 2 * k), idesc,
+                                      (u | b | k) ? 1u : 0u);
+                    umma_commit(&s.kv_empty[st]);
+                }
+            }
+            if (pg_elect()) {
+                umma_commit(&s.s_full[scores & 1u]);
+                if (j + 1 == t.tiles) umma_commit(&s.q_empty);
+            }
+            scores++;
+        };
+        for (int n = 0; alive && next_item(n, t); n++) {
+            if (!t.tiles) continue;
+            if (!wait(&s.q_full, (uint32_t)full)) break;
+            score(0);
+            for (int j = 0; j < t.tiles && alive; j++) {
+                if (j + 1 < t.tiles) score(j + 1);
+                if (!alive || !wait(&s.p_full[sums & 1u], sums >> 1)) break;
+                /* the tile before is out of tensor memory */
+                if (j == 0 && full > 0 && !wait(&s.o_free, (uint32_t)(full - 1))) break;
+                const uint32_t pa = tmem + (sums & 1u) * AP_ROWS;
+                const int keys = min(AP_ROWS, t.keys - j * AP_ROWS);
+                for (int u = 0; u < S::UNITS; u++, unit++) {
+                    const int st = (int)(unit % STAGES);
+                    if (!wait(&s.kv_full[st], unit / STAGES)) break;
+                    const int here = min(max(keys - u * S::V_ROWS, 0), S::V_ROWS);
+                    /* Keys behind the last one that any row sees have weight zero, but their
+                     * values may be anything, and 0 * NaN is not 0: whole steps of 16 of them are left out, the
+                     * rest of the last step is cleared. */
+                    const int steps = (here + 15) / 16;
+                    if (here & 15) {
+                        unsigned char *v = ring + st * S::UNIT_BYTES;
+                        const int rows = steps * 16 - here;
+                        for (int i = lane; i < S::BLOCKS * rows * 8; i += 32) {
+                            const int b = i / (rows * 8), r = i - b * rows * 8;
+                            *reinterpret_cast<uint4 *>(v + b * S::V_ROWS * 128 + here * 128 +
+                                                       r * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    const uint64_t v_desc =
+                        ap_desc_mn(ring_addr + st * S::UNIT_BYTES, S::V_ROWS * 128);
+                    if (pg_elect()) {
+                        for (int k = 0; k < steps; k++)
+                            umma_bf16_ts(tmem + AP_TMEM_O, pa + (u * S::V_ROWS / 16 + k) * 8,
+                                         v_desc + (uint64_t)(k * (16 * 128 / 16)),
+                                         umma_idesc(D) | AP_B_MN, (j | u | k) ? 1u : 0u);
+                        umma_commit(&s.kv_empty[st]);
+                    }
+                }
+                if (!alive) break;
+                if (pg_elect()) umma_commit(&s.pv_done);
+                sums++;
+            }
+            full++;
+        }
+    } else {
+        /* ---------------- softmax and outputs ---------------- */
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int row = quarter * 32 + lane;
+        const int my_token = row / p.a.group, my_head = row - my_token * p.a.group;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const float sc = p.a.scale * LOG2E;
+        uint32_t scores = 0, rounds = 0;     /* steps; exchanges of the two warps of a quarter */
+        bool alive = true;
+        ApItem t = {};
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            alive = alive && pg_wait_warp(bar, parity & 1u, abort_flag, p.status, ST_TMEM_TIMEOUT);
+            tc_fence_after();
+            return alive;
+        };
+        auto exchange = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.pair[quarter]);
+            return wait(&s.pair[quarter], rounds++);
+        };
+        for (int n = 0; alive && next_item(n, t); n++) {
+            const int sees = p.causal ? min(max(t.sees + my_token, 0), t.keys) : t.keys;
+            float top = -INFINITY, sum = 0.0f;            /* top: of scores times sc */
+            const uint32_t before = scores;               /* P V products before this tile */
+            for (int j = 0; j < t.tiles; j++, scores++) {
+                const uint32_t buf = scores & 1u;
+                if (!wait(&s.s_full[buf], scores >> 1)) break;
+                const uint32_t ts = tmem + lanes + buf * AP_ROWS;
+                uint32_t x[2][32];
+                tmem_ld32(ts + half * 64, x[0]);
+                tmem_ld32(ts + half * 64 + 32, x[1]);
+                tmem_ld_wait();
+                const int lim = sees - j * AP_ROWS - half * 64;
+                if (!__all_sync(0xffffffffu, lim >= 64)) {
+#pragma unroll
+                    for (int c = 0; c < 64; c++)
+                        if (c >= lim) x[c >> 5][c & 31] = 0xff800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 64; c++)
+                    mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c >> 5][c & 31]));
+                const uint16_t m16 = (uint16_t)pack_bf16_rn(
+                    fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc, 0.0f);
+                s.top[buf][half][row] = m16;
+                if (!exchange()) break;
+                const float m = fmaxf(bf16_f32(m16), bf16_f32(s.top[buf][half ^ 1][row]));
+                const bool move = m > top + 8.0f || (top == -INFINITY && m > -INFINITY);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float f = move ? exp2_fast(top - m) : 1.0f;
+                    if (move) top = m;
+                    sum *= f;
+                    if (j > 0) {
+                        if (!wait(&s.pv_done, before + j - 1)) break;
+#pragma unroll 1
+                        for (int c = 0; c < D / 2; c += 32) {
+                            const uint32_t to = tmem + lanes + AP_TMEM_O + half * (D / 2) + c;
+                            uint32_t o[32];
+                            tmem_ld32(to, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(to, o);
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                const float base = top == -INFINITY ? 0.0f : top;
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t pk[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float a = exp2_fast(fmaf(__uint_as_float(x[c >> 5][c & 31]), sc, -base)),
+                                b = exp2_fast(
+                                    fmaf(__uint_as_float(x[c >> 5][(c & 31) + 1]), sc, -base));
+                    part[c & 2] += a;
+                    part[(c & 2) + 1] += b;
+                    pk[c >> 1] = pack_bf16_rn(a, b);      /* the weights' one rounding */
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_st32(ts + half * 32, pk);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.p_full[buf]);
+            }
+            if (!alive) break;
+            /* ---- the tile's outputs ---- */
+            const bool real = my_token < t.tokens;
+            const long r = t.token + my_token;
+            const int h = t.head * p.a.group + my_head;
+            uint16_t *out = p.a.out + r * p.a.out_stride + (size_t)h * D + half * (D / 2);
+            if (t.tiles) {
+                s.sum[half][row] = sum;
+                if (!exchange()) break;
+                sum += s.sum[half ^ 1][row];
+                /* A parity tells a phase from the next one only: the last step's scores say that
+                 * the outputs two steps before are done, so the last two are waited for. */
+                if (t.tiles > 1 && !wait(&s.pv_done, before + t.tiles - 2)) break;
+                if (!wait(&s.pv_done, before + t.tiles - 1)) break;
+            }
+            const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+            const uint16_t *gate =
+                p.a.gate ? p.a.gate + r * p.a.gate_stride + (size_t)h * D + half * (D / 2) : nullptr;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 32) {
+                uint32_t o[32];
+                if (t.tiles) {
+                    tmem_ld32(tmem + lanes + AP_TMEM_O + half * (D / 2) + c, o);
+                    tmem_ld_wait();
+                }
+                if (!real) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++)          /* no key: zero, whatever O holds */
+                        y[k] = inv > 0.0f ? __uint_as_float(o[i + k]) * inv : 0.0f;
+                    if (gate) {
+                        const uint4 g = ldg16(gate + c + i);
+                        const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            y[2 * k] *= ad_gate(bf16lo(gw[k]));
+                            y[2 * k + 1] *= ad_gate(bf16hi(gw[k]));
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(out + c + i) =
+                        make_uint4(pack_bf16_rn(y[0], y[1]), pack_bf16_rn(y[2], y[3]),
+                                   pack_bf16_rn(y[4], y[5]), pack_bf16_rn(y[6], y[7]));
+                }
+            }
+            if (p.a.lse && real && half == 0)
+                p.a.lse[r * p.a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+            if (t.tiles) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.o_free);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, AP_TMEM_COLS);
+    }
+}
+
+}  // namespace apus

@@ -23,7 +23,7 @@
 #include <vector>
 
 #include "attn_decode.cuh"
-#include "attn_rows.cuh"
+#include "attn_prompt.cuh"
 #include "attn_view.cuh"
 #include "common.cuh"
 #include "decode_fused.cuh"
@@ -130,7 +130,8 @@ struct Ctx {
     unsigned long long *d_df_timeline = nullptr;   /* [sm_count][DF_MARKS] */
     bool df_timeline_valid = false;
     int ds_absent = -1;
-    /* unfinished results of attention over the paged cache (attn_decode.cuh) */
+    /* unfinished results of attention over the paged cache (attn_decode.cuh); its round counters and
+     * the tile counters of attention over prompts (attn_prompt.cuh) */
     uint2 *d_attn_parts = nullptr;
     unsigned *d_attn_sync = nullptr;
     size_t df_act_elems = 0, df_sa_elems = 0;
@@ -255,8 +256,8 @@ static int ctx_init() {
                      (size_t)c->sm_count * DF_MARKS * sizeof(unsigned long long)));
     CU_OK(cudaMalloc(&c->d_attn_parts, ad_scratch_bytes(c->sm_count)));
     CU_OK(cudaMemset(c->d_attn_parts, 0, ad_scratch_bytes(c->sm_count)));
-    CU_OK(cudaMalloc(&c->d_attn_sync, AD_SYNC_WORDS * sizeof(unsigned)));
-    CU_OK(cudaMemset(c->d_attn_sync, 0, AD_SYNC_WORDS * sizeof(unsigned)));
+    CU_OK(cudaMalloc(&c->d_attn_sync, 2 * AD_SYNC_WORDS * sizeof(unsigned)));
+    CU_OK(cudaMemset(c->d_attn_sync, 0, 2 * AD_SYNC_WORDS * sizeof(unsigned)));
     g_apus_use_pdl = env_long("APUS_CUDA_PDL", 1) != 0;
     g_pg_overlap = (int)env_long("APUS_CUDA_GEMM_OVERLAP", 1);
     g_pg_dynamic = (int)env_long("APUS_CUDA_GEMM_DYNAMIC", 3);
