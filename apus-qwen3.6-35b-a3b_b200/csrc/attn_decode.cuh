@@ -199,14 +199,14 @@ __device__ __forceinline__ void ad_merge(float &top, float &sum, float4 &acc, fl
 /* four values of a head's sums as they leave */
 __device__ __forceinline__ void ad_finish4(const AttnView &a, long row, int head, int D, int c,
                                            float4 acc, float top, float sum) {
-    const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
     acc.x *= inv;
     acc.y *= inv;
     acc.z *= inv;
     acc.w *= inv;
     ad_store4(a, row, head * D + c, acc);
     if (c == 0 && a.lse)
-        a.lse[row * a.heads + head] = sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+        a.lse[row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 __device__ __forceinline__ void ad_put2(uint2 *at, float x, float y, unsigned round) {
     asm volatile("st.relaxed.gpu.global.v4.u32 [%0], {%1, %2, %3, %2};" ::"l"(at),
@@ -540,10 +540,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             const int h0 = cc.head * group;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const float inv = l[n] > 0.0f ? __fdividef(1.0f, l[n]) : 0.0f;
+                const float inv = l[n] == 0.0f ? 0.0f : __fdividef(1.0f, l[n]);
                 if (p.a.lse && t4 == 0 && n * 8 + g < group)
                     p.a.lse[row * p.a.heads + h0 + n * 8 + g] =
-                        l[n] > 0.0f ? (m[n] + log2f(l[n])) * LN2 : -INFINITY;
+                        l[n] == 0.0f ? -INFINITY : (m[n] + log2f(l[n])) * LN2;
                 const float v0 = __shfl_sync(0xffffffffu, inv, t4 * 8),
                             v1 = __shfl_sync(0xffffffffu, inv, t4 * 8 + 4);
                 /* the accumulators hold (value g; heads 2 t, 2 t + 1); memory wants (head g;

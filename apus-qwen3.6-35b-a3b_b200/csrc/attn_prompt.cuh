@@ -9,7 +9,7 @@
  * every key is fetched once for all its heads, and the causal edge costs few masked scores.
  *
  * One persistent CTA per SM takes such tiles from a counter (the last tiles of each sequence
- * first: they see the most keys).  Ten warps:
+ * first: they see the most keys).  Its warps:
  *   warp 0     finds the tile's sequence, loads Q (64 KB at head_dim 256) and a ring of 32 KB pieces of K and V
  *   warp 1     issues tcgen05.mma: S(j+1) before O += P(j) V(j), so that the tensor cores work
  *              while the softmax of a tile runs
@@ -75,7 +75,7 @@ struct ApItem {
     int sees;                                /* keys that the first token sees */
 };
 struct ApShared {
-    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done, o_free;
+    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free;
     uint64_t item_full[AP_ITEMS], item_empty[AP_ITEMS], pair[4];
     ApItem item[AP_ITEMS];
     uint32_t tmem;
@@ -182,7 +182,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
     extern __shared__ __align__(1024) unsigned char ap_smem[];
     unsigned char *q_smem = ap_smem, *ring = ap_smem + S::Q_BYTES;
     ApShared &s = *reinterpret_cast<ApShared *>(ring + STAGES * S::UNIT_BYTES);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   /* known to be the warp's */
     if (smem_u32(ap_smem) & 1023) {          /* swizzled tiles: the same answer in all threads */
         if (tid == 0) set_status(p.status, ST_BAD_INDEX);
         return;
@@ -197,8 +198,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1);
             mbar_init(&s.p_full[i], AP_SOFT_WARPS);
+            mbar_init(&s.pv_done[i], 1);
         }
-        mbar_init(&s.pv_done, 1);
         mbar_init(&s.o_free, AP_SOFT_WARPS);
         for (int i = 0; i < AP_ITEMS; i++) {
             mbar_init(&s.item_full[i], 1);
@@ -222,7 +223,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         if (!pg_wait(&s.item_full[i], (uint32_t)(n / AP_ITEMS) & 1u, abort_flag, p.status,
                      ST_SCHED_TIMEOUT))
             return false;
-        t = s.item[i];
+        /* by shuffles, so that what follows from it (loops, descriptors) is known to be the
+         * same in all lanes and is kept in uniform registers, where MMAs want it */
+        const int *from = reinterpret_cast<const int *>(&s.item[i]);
+        int *to = reinterpret_cast<int *>(&t);
+#pragma unroll
+        for (int w = 0; w < (int)(sizeof(ApItem) / 4); w++)
+            to[w] = __shfl_sync(0xffffffffu, from[w], 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.item_empty[i]);
         return t.tokens >= 0;
@@ -325,6 +332,19 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             tc_fence_after();
             return alive;
         };
+        /* A wait costs this warp about 170 cycles even where there is nothing to wait for, and the
+         * tensor cores have one or two MMAs queued meanwhile: a barrier is looked at before the
+         * MMAs that come before it are issued, and waited for only where that said no. */
+        bool unit_ready = false, weights_ready = false;
+        auto wait_seen = [&](bool seen, uint64_t *bar, uint32_t parity) {
+            if (!__all_sync(0xffffffffu, seen)) return wait(bar, parity);
+            tc_fence_after();
+            return alive;
+        };
+        auto look_ahead = [&]() {            /* at the piece after this one */
+            const uint32_t next = unit + 1;
+            unit_ready = mbar_test(&s.kv_full[next % STAGES], (next / STAGES) & 1u);
+        };
         auto score = [&](int j) {
             const uint32_t d = tmem + (scores & 1u) * AP_ROWS;
             /* no more columns than there are keys (what lies behind them is masked) */
@@ -332,7 +352,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             const uint32_t idesc = umma_idesc(cols);
             for (int u = 0; u < S::UNITS; u++, unit++) {
                 const int st = (int)(unit % STAGES);
-                if (!wait(&s.kv_full[st], unit / STAGES)) return;
+                if (!wait_seen(unit_ready, &s.kv_full[st], unit / STAGES)) return;
+                look_ahead();
+                if (u + 1 == S::UNITS)
+                    weights_ready = mbar_test(&s.p_full[sums & 1u], (sums >> 1) & 1u);
                 const uint64_t k_desc = umma_smem_desc(ring_addr + st * S::UNIT_BYTES);
                 if (pg_elect()) {
 #pragma unroll
@@ -358,15 +381,17 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             if (!wait(&s.q_full, (uint32_t)full)) break;
             score(0);
             for (int j = 0; j < t.tiles && alive; j++) {
+                weights_ready = false;
                 if (j + 1 < t.tiles) score(j + 1);
-                if (!alive || !wait(&s.p_full[sums & 1u], sums >> 1)) break;
+                if (!alive || !wait_seen(weights_ready, &s.p_full[sums & 1u], sums >> 1)) break;
                 /* the tile before is out of tensor memory */
                 if (j == 0 && full > 0 && !wait(&s.o_free, (uint32_t)(full - 1))) break;
                 const uint32_t pa = tmem + (sums & 1u) * AP_ROWS;
                 const int keys = min(AP_ROWS, t.keys - j * AP_ROWS);
                 for (int u = 0; u < S::UNITS; u++, unit++) {
                     const int st = (int)(unit % STAGES);
-                    if (!wait(&s.kv_full[st], unit / STAGES)) break;
+                    if (!wait_seen(unit_ready, &s.kv_full[st], unit / STAGES)) break;
+                    look_ahead();
                     const int here = min(max(keys - u * S::V_ROWS, 0), S::V_ROWS);
                     /* Keys behind the last one that any row sees have weight zero, but their
                      * values may be anything, and 0 * NaN is not 0: whole steps of 16 of them are left out, the
@@ -386,15 +411,17 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     const uint64_t v_desc =
                         ap_desc_mn(ring_addr + st * S::UNIT_BYTES, S::V_ROWS * 128);
                     if (pg_elect()) {
-                        for (int k = 0; k < steps; k++)
-                            umma_bf16_ts(tmem + AP_TMEM_O, pa + (u * S::V_ROWS / 16 + k) * 8,
-                                         v_desc + (uint64_t)(k * (16 * 128 / 16)),
-                                         umma_idesc(D) | AP_B_MN, (j | u | k) ? 1u : 0u);
+#pragma unroll
+                        for (int k = 0; k < S::V_ROWS / 16; k++)
+                            if (k < steps)
+                                umma_bf16_ts(tmem + AP_TMEM_O, pa + (u * S::V_ROWS / 16 + k) * 8,
+                                             v_desc + (uint64_t)(k * (16 * 128 / 16)),
+                                             umma_idesc(D) | AP_B_MN, (j | u | k) ? 1u : 0u);
                         umma_commit(&s.kv_empty[st]);
                     }
                 }
                 if (!alive) break;
-                if (pg_elect()) umma_commit(&s.pv_done);
+                if (pg_elect()) umma_commit(&s.pv_done[sums & 1u]);
                 sums++;
             }
             full++;
@@ -420,10 +447,25 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             if (lane == 0) mbar_arrive(&s.pair[quarter]);
             return wait(&s.pair[quarter], rounds++);
         };
+        /* O holds step i.  A parity tells a phase only from the one before it, and i's scores, which
+         * this warp has seen, say no more than that step i - 2 is through: two barriers in turn. */
+        auto wait_outputs = [&](uint32_t i) { return wait(&s.pv_done[i & 1u], i >> 1); };
         for (int n = 0; alive && next_item(n, t); n++) {
             const int sees = p.causal ? min(max(t.sees + my_token, 0), t.keys) : t.keys;
+            const bool real = my_token < t.tokens;
+            const long r = t.token + my_token;
+            const int h = t.head * p.a.group + my_head;
+            uint16_t *out = p.a.out + r * p.a.out_stride + (size_t)h * D + half * (D / 2);
+            /* (rows that are none read the first row's and store nothing) */
+            const uint16_t *my_gate = p.a.gate;
+            if (p.a.gate)
+                my_gate += (real ? r : (long)t.token) * p.a.gate_stride + (size_t)h * D +
+                           half * (D / 2);
+            if (p.a.gate)
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 64)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(my_gate + c));
             float top = -INFINITY, sum = 0.0f;            /* top: of scores times sc */
-            const uint32_t before = scores;               /* P V products before this tile */
             for (int j = 0; j < t.tiles; j++, scores++) {
                 const uint32_t buf = scores & 1u;
                 if (!wait(&s.s_full[buf], scores >> 1)) break;
@@ -453,7 +495,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     if (move) top = m;
                     sum *= f;
                     if (j > 0) {
-                        if (!wait(&s.pv_done, before + j - 1)) break;
+                        if (!wait_outputs(scores - 1)) break;
 #pragma unroll 1
                         for (int c = 0; c < D / 2; c += 32) {
                             const uint32_t to = tmem + lanes + AP_TMEM_O + half * (D / 2) + c;
@@ -489,38 +531,37 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             if (!alive) break;
             /* ---- the tile's outputs ---- */
-            const bool real = my_token < t.tokens;
-            const long r = t.token + my_token;
-            const int h = t.head * p.a.group + my_head;
-            uint16_t *out = p.a.out + r * p.a.out_stride + (size_t)h * D + half * (D / 2);
+            constexpr int CHUNKS = D / 64;                /* of 32 values */
+            uint4 gate[2][4];                             /* two of them, the first under way now */
+            auto load_gate = [&](int c) {
+                if (p.a.gate)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) gate[c & 1][i] = ldg16(my_gate + c * 32 + i * 8);
+            };
+#pragma unroll
+            for (int c = 0; c < 2 && c < CHUNKS; c++) load_gate(c);
             if (t.tiles) {
                 s.sum[half][row] = sum;
                 if (!exchange()) break;
                 sum += s.sum[half ^ 1][row];
-                /* A parity tells a phase from the next one only: the last step's scores say that
-                 * the outputs two steps before are done, so the last two are waited for. */
-                if (t.tiles > 1 && !wait(&s.pv_done, before + t.tiles - 2)) break;
-                if (!wait(&s.pv_done, before + t.tiles - 1)) break;
+                if (!wait_outputs(scores - 1)) break;
             }
-            const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
-            const uint16_t *gate =
-                p.a.gate ? p.a.gate + r * p.a.gate_stride + (size_t)h * D + half * (D / 2) : nullptr;
-#pragma unroll 1
-            for (int c = 0; c < D / 2; c += 32) {
+            const float inv = __fdividef(1.0f, sum);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++) {
                 uint32_t o[32];
                 if (t.tiles) {
-                    tmem_ld32(tmem + lanes + AP_TMEM_O + half * (D / 2) + c, o);
+                    tmem_ld32(tmem + lanes + AP_TMEM_O + half * (D / 2) + c * 32, o);
                     tmem_ld_wait();
                 }
-                if (!real) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
+                for (int i = 0; i < 4; i++) {
                     float y[8];
 #pragma unroll
                     for (int k = 0; k < 8; k++)          /* no key: zero, whatever O holds */
-                        y[k] = inv > 0.0f ? __uint_as_float(o[i + k]) * inv : 0.0f;
-                    if (gate) {
-                        const uint4 g = ldg16(gate + c + i);
+                        y[k] = sum == 0.0f ? 0.0f : __uint_as_float(o[i * 8 + k]) * inv;
+                    if (p.a.gate) {
+                        const uint4 g = gate[c & 1][i];
                         const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
@@ -528,13 +569,15 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                             y[2 * k + 1] *= ad_gate(bf16hi(gw[k]));
                         }
                     }
-                    *reinterpret_cast<uint4 *>(out + c + i) =
-                        make_uint4(pack_bf16_rn(y[0], y[1]), pack_bf16_rn(y[2], y[3]),
-                                   pack_bf16_rn(y[4], y[5]), pack_bf16_rn(y[6], y[7]));
+                    const uint4 v = make_uint4(pack_bf16_rn(y[0], y[1]), pack_bf16_rn(y[2], y[3]),
+                                               pack_bf16_rn(y[4], y[5]), pack_bf16_rn(y[6], y[7]));
+                    if (real) *reinterpret_cast<uint4 *>(out + c * 32 + i * 8) = v;
                 }
+                __syncwarp();
+                if (c + 2 < CHUNKS) load_gate(c + 2);
             }
             if (p.a.lse && real && half == 0)
-                p.a.lse[r * p.a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+                p.a.lse[r * p.a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
             if (t.tiles) {
                 tc_fence_before();
                 __syncwarp();

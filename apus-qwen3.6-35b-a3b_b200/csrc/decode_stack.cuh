@@ -142,19 +142,6 @@ __device__ __forceinline__ bool ds_spin(const unsigned int *p, unsigned int targ
     return false;
 }
 
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 
 /* A lane's share of a row's 128-k slice: 16 bytes of each of its four 64-byte windows, which
  * are the operands of two k steps each.  p: the row's slice + (lane & 3) * 16. */
