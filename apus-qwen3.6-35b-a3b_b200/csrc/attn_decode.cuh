@@ -148,8 +148,13 @@ struct AdCursor {
 };
 
 /* o narrowed once, the gate included (its sigmoid to a few 2^-23: no step of a BF16 result) */
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float ad_gate(float g) {
-    return __fdividef(1.0f, 1.0f + __expf(-g));
+    return rcp_fast(1.0f + exp2_fast(-LOG2E * g));
 }
 /* an 8 x 8 tile of 16-bit values, two to a lane, the other way round */
 __device__ __forceinline__ uint32_t ad_transpose(uint32_t x) {

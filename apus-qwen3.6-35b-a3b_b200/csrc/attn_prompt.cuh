@@ -12,26 +12,28 @@
  * first: they see the most keys).  Its warps:
  *   warp 0     finds the tile's sequence, loads Q (64 KB at head_dim 256) and a ring of 32 KB pieces of K and V
  *   warp 1     issues tcgen05.mma: S(j+1) before O += P(j) V(j), so that the tensor cores work
- *              while the softmax of a tile runs
- *   warps 2-9  softmax: two warps to each quarter of the rows, each half of the 128 scores of a
- *              row; outputs at the end
- * S is double-buffered in tensor memory (2 x 128 columns), O takes head_dim columns.  P stays
- * there as well: narrowed to BF16 it overwrites its own scores and is the MMA's A operand, so that
- * shared memory carries Q, K and V only.  (K and Q are K-major; V's rows are its K dimension: the
- * MN-major form of the same 128B-swizzled tile.)
+ *              while the softmax of a step of 128 keys runs
+ *   warps 4-11 softmax, two warps to each quarter of the rows with half of the 128 scores each;
+ *              outputs at the end
+ * S is double-buffered in tensor memory (2 x 128 columns), O takes head_dim columns.  P stays there as well: narrowed to
+ * BF16 it overwrites its own scores and is the MMA's A operand, so that shared memory carries Q, K and
+ * V only.  (K and Q are K-major; V's rows are its K dimension: the MN-major form of the same
+ * 128B-swizzled tile.)
  *
  * The maximum that a row's weights are taken against moves only when a score is 2^8 above it: any
  * reference within the range of fp32 and BF16 gives the same quotient, and O in tensor memory
- * is then hardly ever scaled again (that takes its 256 columns through registers).
+ * is then hardly ever scaled again (that takes its columns through registers).
  *
- * Bound at head_dim 256 and long prompts: the MMAs, 2048 cycles for 128 keys, beside 1024 of
- * exponentials (16 a cycle and SM) on other units; at 128 and 64 the exponentials (1024
- * against 1024 and 512).
+ * Bound at head_dim 256 and long prompts: shared memory (Q and K for S, V, and what TMA writes:
+ * 2560 cycles for 128 keys) beside 2048 of MMAs and 1024 of exponentials (16 a cycle and SM); at
+ * 128 the same at half the size, 1280 beside 1024 and 1024; at 64 the exponentials.
  */
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "attn_decode.cuh"
 #include "attn_view.cuh"
@@ -42,7 +44,11 @@ namespace apus {
 
 constexpr int AP_ROWS = 128;                 /* rows of a tile, keys of a step */
 constexpr int AP_SOFT_WARPS = 8;
-constexpr int AP_THREADS = 64 + AP_SOFT_WARPS * 32;
+constexpr int AP_THREADS = 128 + AP_SOFT_WARPS * 32;
+/* The registers of a block of twelve warps are 168 a thread.  The two warps that issue loads and
+ * MMAs (and two that only fill up their group) need few; the softmax warps take over the rest:
+ * 128 x 64 + 256 x 216 <= 384 x 168. */
+constexpr int AP_REGS_ISSUE = 40, AP_REGS_SOFT = 232;
 constexpr int AP_TMEM_COLS = 512;
 constexpr int AP_TMEM_O = 256;               /* scores in columns 0..255 */
 constexpr int AP_ITEMS = 2;
@@ -97,16 +103,34 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
-/* D[tmem] (+)= A[tmem] * B[smem] */
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                             uint32_t idesc, uint32_t accumulate) {
+/* D[tmem] (+)= A[smem] * B[smem] and A[tmem] * B[smem].  Of a descriptor only the low word, with
+ * the address, changes from one MMA to the next. */
+__device__ __forceinline__ void ap_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
+                                          uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                          uint32_t accumulate) {
     asm volatile(
         "{\n\t"
         ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        ".reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %2};\n\t"
+        "mov.b64 b, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
         "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ap_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+                                          uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -124,6 +148,104 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+/* 16 rows x 8 columns at a time: lane 4 g + t has columns 2 t, 2 t + 1 of rows g and g + 8 */
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+/* two fp32 operations in one instruction */
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+/* 2^x of two values on the FMA units, beside the 16 a cycle of the special function units:
+ * x = n + f with f in [-1/2, 1/2] (n by adding 1.5 * 2^23, whose last bits are then n), 2^f by
+ * its polynomial of degree 5 with the smallest largest relative error there (7.5e-8, fitted by
+ * reweighted least squares), and n in the exponent of a factor.  x in [-126, 127], others as
+ * the nearer end; NaN stays. */
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+    const float2 big = make_float2(12582912.0f, 12582912.0f);
+    const float2 t = add2(x, big);
+    const float2 n = add2(t, make_float2(-12582912.0f, -12582912.0f));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 y = make_float2(1.3276466634124517e-3f, 1.3276466634124517e-3f);
+    y = fma2(y, f, make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
+    y = fma2(y, f, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
+    y = fma2(y, f, make_float2(2.4022120237350464e-1f, 2.4022120237350464e-1f));
+    y = fma2(y, f, make_float2(6.931469440460205e-1f, 6.931469440460205e-1f));
+    y = fma2(y, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    /* (1.5 * 2^23's own bits are shifted out) */
+    return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) * 0x800000u + 0x3f800000u),
+                               __uint_as_float(__float_as_uint(t.y) * 0x800000u + 0x3f800000u)));
+}
+/* Four lanes with four pairs each: pair w of lane t to lane w, as its pair t. */
+__device__ __forceinline__ void ap_turn(uint32_t (&e)[4][2], int t) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const bool odd = t & 1, high = t & 2;
+        const uint32_t x = __shfl_xor_sync(0xffffffffu, odd ? e[0][k] : e[1][k], 1),
+                       y = __shfl_xor_sync(0xffffffffu, odd ? e[2][k] : e[3][k], 1);
+        const uint32_t a0 = odd ? x : e[0][k], a1 = odd ? e[1][k] : x, a2 = odd ? y : e[2][k],
+                       a3 = odd ? e[3][k] : y;
+        const uint32_t u = __shfl_xor_sync(0xffffffffu, high ? a0 : a2, 2),
+                       v = __shfl_xor_sync(0xffffffffu, high ? a1 : a3, 2);
+        e[0][k] = high ? u : a0;
+        e[1][k] = high ? v : a1;
+        e[2][k] = high ? a2 : u;
+        e[3][k] = high ? a3 : v;
+    }
 }
 /* B whose N dimension is contiguous (V: keys are K): 64 values x 8 keys to a swizzle atom of
  * 1024 bytes, the next 8 keys SBO behind it, the next 64 values LBO */
@@ -235,6 +357,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         return t.tokens >= 0;
     };
 
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AP_REGS_ISSUE));
     if (warp == 0) {
         /* ---------------- tiles and loads ---------------- */
         uint32_t unit = 0;
@@ -325,6 +449,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         int full = 0;
         bool alive = true;
         const uint64_t q_desc = umma_smem_desc(smem_u32(q_smem));
+        const uint32_t q_lo = (uint32_t)q_desc, q_hi = (uint32_t)(q_desc >> 32);
         const uint32_t ring_addr = smem_u32(ring);
         ApItem t = {};
         auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -356,17 +481,17 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 look_ahead();
                 if (u + 1 == S::UNITS)
                     weights_ready = mbar_test(&s.p_full[sums & 1u], (sums >> 1) & 1u);
-                const uint64_t k_desc = umma_smem_desc(ring_addr + st * S::UNIT_BYTES);
+                const uint32_t k_lo = (uint32_t)umma_smem_desc(ring_addr + st * S::UNIT_BYTES);
+                const uint32_t q_at = q_lo + u * S::K_BLOCKS * (AP_ROWS * 128 / 16);
                 if (pg_elect()) {
 #pragma unroll
                     for (int b = 0; b < S::K_BLOCKS; b++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            umma_bf16(d,
-                                      q_desc + (uint64_t)((u * S::K_BLOCKS + b) * (AP_ROWS * 128 / 16) +
-                                                          2 * k),
-                                      k_desc + (uint64_t)(b * (AP_ROWS * 128 / 16) + 2 * k), idesc,
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t off = b * (AP_ROWS * 128 / 16) + 2 * k;
+                            ap_mma_ss(d, q_at + off, q_hi, k_lo + off, q_hi, idesc,
                                       (u | b | k) ? 1u : 0u);
+                        }
                     umma_commit(&s.kv_empty[st]);
                 }
             }
@@ -410,13 +535,15 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     }
                     const uint64_t v_desc =
                         ap_desc_mn(ring_addr + st * S::UNIT_BYTES, S::V_ROWS * 128);
+                    const uint32_t v_lo = (uint32_t)v_desc, v_hi = (uint32_t)(v_desc >> 32);
                     if (pg_elect()) {
 #pragma unroll
                         for (int k = 0; k < S::V_ROWS / 16; k++)
                             if (k < steps)
-                                umma_bf16_ts(tmem + AP_TMEM_O, pa + (u * S::V_ROWS / 16 + k) * 8,
-                                             v_desc + (uint64_t)(k * (16 * 128 / 16)),
-                                             umma_idesc(D) | AP_B_MN, (j | u | k) ? 1u : 0u);
+                                ap_mma_ts(tmem + AP_TMEM_O, pa + (u * S::V_ROWS / 16 + k) * 8,
+                                          v_lo + k * (16 * 128 / 16), v_hi,
+                                          umma_idesc(D) | AP_B_MN,
+                                          (j | u | k) ? 1u : 0u);
                         umma_commit(&s.kv_empty[st]);
                     }
                 }
@@ -426,14 +553,19 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             full++;
         }
+    }
     } else {
         /* ---------------- softmax and outputs ---------------- */
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AP_REGS_SOFT));
+        constexpr int COLS = AP_ROWS / 2;    /* scores of a row that a thread has */
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
         const int row = quarter * 32 + lane;
-        const int my_token = row / p.a.group, my_head = row - my_token * p.a.group;
+        /* row / group as a product (rows below 128, groups up to 16) */
+        const int by_group = 65536 / p.a.group + 1;
+        const int my_token = (row * by_group) >> 16, my_head = row - my_token * p.a.group;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const float sc = p.a.scale * LOG2E;
-        uint32_t scores = 0, rounds = 0;     /* steps; exchanges of the two warps of a quarter */
+        uint32_t first = 0, rounds = 0;      /* steps before this tile; exchanges of a pair of warps */
         bool alive = true;
         ApItem t = {};
         auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -447,42 +579,40 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             if (lane == 0) mbar_arrive(&s.pair[quarter]);
             return wait(&s.pair[quarter], rounds++);
         };
-        /* O holds step i.  A parity tells a phase only from the one before it, and i's scores, which
-         * this warp has seen, say no more than that step i - 2 is through: two barriers in turn. */
+        /* O holds step i.  A parity tells a phase only from the one before it, and that this warp
+         * (or its pair) has seen i's scores says no more than that step i - 2 is through: two
+         * barriers in turn. */
         auto wait_outputs = [&](uint32_t i) { return wait(&s.pv_done[i & 1u], i >> 1); };
         for (int n = 0; alive && next_item(n, t); n++) {
             const int sees = p.causal ? min(max(t.sees + my_token, 0), t.keys) : t.keys;
             const bool real = my_token < t.tokens;
             const long r = t.token + my_token;
             const int h = t.head * p.a.group + my_head;
-            uint16_t *out = p.a.out + r * p.a.out_stride + (size_t)h * D + half * (D / 2);
-            /* (rows that are none read the first row's and store nothing) */
-            const uint16_t *my_gate = p.a.gate;
-            if (p.a.gate)
-                my_gate += (real ? r : (long)t.token) * p.a.gate_stride + (size_t)h * D +
-                           half * (D / 2);
-            if (p.a.gate)
+            if (p.a.gate && real)                         /* to L2, for the end of the tile */
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 64)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(my_gate + c));
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                        p.a.gate + r * p.a.gate_stride + (size_t)h * D + half * (D / 2) + c));
             float top = -INFINITY, sum = 0.0f;            /* top: of scores times sc */
-            for (int j = 0; j < t.tiles; j++, scores++) {
-                const uint32_t buf = scores & 1u;
-                if (!wait(&s.s_full[buf], scores >> 1)) break;
+            for (int j = 0; j < t.tiles; j++) {
+                const uint32_t step = first + j, buf = step & 1u;
+                if (!wait(&s.s_full[buf], step >> 1)) break;
                 const uint32_t ts = tmem + lanes + buf * AP_ROWS;
-                uint32_t x[2][32];
-                tmem_ld32(ts + half * 64, x[0]);
-                tmem_ld32(ts + half * 64 + 32, x[1]);
-                tmem_ld_wait();
-                const int lim = sees - j * AP_ROWS - half * 64;
-                if (!__all_sync(0xffffffffu, lim >= 64)) {
+                uint32_t x[COLS / 32][32];
 #pragma unroll
-                    for (int c = 0; c < 64; c++)
+                for (int c = 0; c < COLS / 32; c++)
+                    tmem_ld32(ts + half * COLS + c * 32, x[c]);
+                tmem_ld_wait();
+                const int lim = sees - j * AP_ROWS - half * COLS;
+                const bool masked = !__all_sync(0xffffffffu, lim >= COLS);
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < COLS; c++)
                         if (c >= lim) x[c >> 5][c & 31] = 0xff800000u;
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 64; c++)
+                for (int c = 0; c < COLS; c++)
                     mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c >> 5][c & 31]));
                 const uint16_t m16 = (uint16_t)pack_bf16_rn(
                     fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc, 0.0f);
@@ -495,86 +625,144 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     if (move) top = m;
                     sum *= f;
                     if (j > 0) {
-                        if (!wait_outputs(scores - 1)) break;
+                        if (!wait_outputs(step - 1)) break;
+                        const uint32_t to = tmem + lanes + AP_TMEM_O + half * (D / 2);
 #pragma unroll 1
                         for (int c = 0; c < D / 2; c += 32) {
-                            const uint32_t to = tmem + lanes + AP_TMEM_O + half * (D / 2) + c;
                             uint32_t o[32];
-                            tmem_ld32(to, o);
+                            tmem_ld32(to + c, o);
                             tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 32; i++)
                                 o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(to, o);
+                            tmem_st32(to + c, o);
                         }
                         tmem_st_wait();
                     }
                 }
                 const float base = top == -INFINITY ? 0.0f : top;
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t pk[32];
+                const float2 sc2 = make_float2(sc, sc), base2 = make_float2(-base, -base);
+                float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                /* Up to head_dim 128 the exponentials are what bounds a step: every POLY-th pair
+                 * goes to the FMA units.  (Where scores are masked their weight has to be 0.) */
+                constexpr int POLY = D == 256 ? 0 : 4;
+                auto weights = [&](auto some_poly) {
 #pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    const float a = exp2_fast(fmaf(__uint_as_float(x[c >> 5][c & 31]), sc, -base)),
-                                b = exp2_fast(
-                                    fmaf(__uint_as_float(x[c >> 5][(c & 31) + 1]), sc, -base));
-                    part[c & 2] += a;
-                    part[(c & 2) + 1] += b;
-                    pk[c >> 1] = pack_bf16_rn(a, b);      /* the weights' one rounding */
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_st32(ts + half * 32, pk);
+                    for (int c = 0; c < COLS / 32; c++) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float2 z = fma2(make_float2(__uint_as_float(x[c][2 * i]),
+                                                              __uint_as_float(x[c][2 * i + 1])),
+                                                  sc2, base2);
+                            const bool poly = some_poly.value && i % (POLY ? POLY : 1) == POLY - 1;
+                            const float2 w = poly ? exp2_poly(z)
+                                                  : make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                            part[i & 1] = add2(part[i & 1], w);
+                            pk[i] = pack_bf16_rn(w.x, w.y);       /* the weights' one rounding */
+                        }
+                        tmem_st16(ts + half * (COLS / 2) + c * 16, pk);
+                    }
+                };
+                if (POLY && !masked) weights(std::true_type());
+                else weights(std::false_type());
+                part[0] = add2(part[0], part[1]);
+                sum += part[0].x + part[0].y;
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.p_full[buf]);
             }
             if (!alive) break;
-            /* ---- the tile's outputs ---- */
-            constexpr int CHUNKS = D / 64;                /* of 32 values */
-            uint4 gate[2][4];                             /* two of them, the first under way now */
-            auto load_gate = [&](int c) {
-                if (p.a.gate)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) gate[c & 1][i] = ldg16(my_gate + c * 32 + i * 8);
+            /* ---- the tile's outputs ----
+             * Read from tensor memory as 16 rows x 8 values a step, four lanes to a row with two
+             * values each: after a 4 x 4 exchange a lane has 8 values side by side, and a
+             * warp's load or store is 64 bytes of each of 8 rows (a row to a lane would be 32 lines
+             * an instruction).  The loop stays one: unrolled, its instructions took longer to
+             * come than to run (12000 cycles a tile). */
+            constexpr int CHUNK = D / 2 < 64 ? D / 2 : 64, PIECES = CHUNK / 32;
+            constexpr int CHUNKS = D / 2 / CHUNK;         /* steps for each 16 rows */
+            const int t4 = lane & 3, g = lane >> 2;
+            auto place = [&](int i, int k, long &token, int &in) {
+                const int o_row = quarter * 32 + (i / CHUNKS) * 16 + k * 8 + g;
+                const int in_tile = (o_row * by_group) >> 16;
+                token = t.token + in_tile;
+                in = (t.head * p.a.group + o_row - in_tile * p.a.group) * D + half * (D / 2) +
+                     (i % CHUNKS) * CHUNK + t4 * 8;
+                return in_tile < t.tokens;
             };
+            uint4 gate[2][PIECES];                        /* of the next step, under way */
+            auto load_gate = [&](int i) {
 #pragma unroll
-            for (int c = 0; c < 2 && c < CHUNKS; c++) load_gate(c);
+                for (int k = 0; k < 2; k++) {
+                    long token;
+                    int in;
+                    if (place(i, k, token, in))
+#pragma unroll
+                        for (int w = 0; w < PIECES; w++)
+                            gate[k][w] = ldg16(p.a.gate + token * p.a.gate_stride + in + w * 32);
+                }
+                __syncwarp();
+            };
+            if (p.a.gate) load_gate(0);
             if (t.tiles) {
                 s.sum[half][row] = sum;
                 if (!exchange()) break;
                 sum += s.sum[half ^ 1][row];
-                if (!wait_outputs(scores - 1)) break;
+                if (!wait_outputs(first + t.tiles - 1)) break;
             }
             const float inv = __fdividef(1.0f, sum);
+#pragma unroll 1
+            for (int i = 0; i < 2 * CHUNKS; i++) {
+                uint4 now[2][PIECES];
 #pragma unroll
-            for (int c = 0; c < CHUNKS; c++) {
-                uint32_t o[32];
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int w = 0; w < PIECES; w++) now[k][w] = gate[k][w];
+                if (p.a.gate && i + 1 < 2 * CHUNKS) load_gate(i + 1);
+                uint32_t o[CHUNK / 2];
                 if (t.tiles) {
-                    tmem_ld32(tmem + lanes + AP_TMEM_O + half * (D / 2) + c * 32, o);
+                    tmem_ld_16x256(tmem + lanes + ((uint32_t)(i / CHUNKS * 16) << 16) + AP_TMEM_O +
+                                       half * (D / 2) + (i % CHUNKS) * CHUNK,
+                                   o);
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float y[8];
+                for (int k = 0; k < 2; k++) {
+                    long token;
+                    int in;
+                    const bool there = place(i, k, token, in);
+                    const int from = (i / CHUNKS) * 16 + k * 8 + g;
+                    const float f = __shfl_sync(0xffffffffu, inv, from);
+                    const float2 f2 = make_float2(f, f);
+                    const bool none = __shfl_sync(0xffffffffu, sum, from) == 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 8; k++)          /* no key: zero, whatever O holds */
-                        y[k] = sum == 0.0f ? 0.0f : __uint_as_float(o[i * 8 + k]) * inv;
-                    if (p.a.gate) {
-                        const uint4 g = gate[c & 1][i];
-                        const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+                    for (int w = 0; w < PIECES; w++) {
+                        uint32_t e[4][2];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            y[2 * k] *= ad_gate(bf16lo(gw[k]));
-                            y[2 * k + 1] *= ad_gate(bf16hi(gw[k]));
+                        for (int x = 0; x < 4; x++) {
+                            e[x][0] = o[(w * 4 + x) * 4 + k * 2];
+                            e[x][1] = o[(w * 4 + x) * 4 + k * 2 + 1];
                         }
+                        ap_turn(e, t4);
+                        uint32_t v[4];
+                        const uint32_t z[4] = {now[k][w].x, now[k][w].y, now[k][w].z, now[k][w].w};
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            float2 y = mul2(make_float2(__uint_as_float(e[x][0]),
+                                                        __uint_as_float(e[x][1])), f2);
+                            if (p.a.gate)
+                                y = mul2(y, make_float2(ad_gate(bf16lo(z[x])), ad_gate(bf16hi(z[x]))));
+                            /* no key: zero, whatever O holds */
+                            v[x] = none ? 0u : pack_bf16_rn(y.x, y.y);
+                        }
+                        if (there)
+                            *reinterpret_cast<uint4 *>(p.a.out + token * p.a.out_stride + in +
+                                                       w * 32) =
+                                make_uint4(v[0], v[1], v[2], v[3]);
                     }
-                    const uint4 v = make_uint4(pack_bf16_rn(y[0], y[1]), pack_bf16_rn(y[2], y[3]),
-                                               pack_bf16_rn(y[4], y[5]), pack_bf16_rn(y[6], y[7]));
-                    if (real) *reinterpret_cast<uint4 *>(out + c * 32 + i * 8) = v;
                 }
                 __syncwarp();
-                if (c + 2 < CHUNKS) load_gate(c + 2);
             }
             if (p.a.lse && real && half == 0)
                 p.a.lse[r * p.a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
@@ -583,6 +771,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.o_free);
             }
+            first += t.tiles;
         }
     }
     tc_fence_before();
