@@ -338,6 +338,9 @@ static int launch_prompt(Ctx *c, const PromptParams &p, const ApusCudaAttnKeys *
     const int grid = p.items < c->sm_count ? p.items : c->sm_count;
     LAUNCH_OK(launch_k(attn_prompt_kernel<D>, dim3(grid), dim3(AP_THREADS), smem, st, mq, mk, mv,
                        p));
+    if (p.splits > 1)
+        LAUNCH_OK(launch_k(attn_prompt_join_kernel<D>, dim3(p.items / p.splits, 4), dim3(256), 0,
+                           st, p));
     return 0;
 }
 
@@ -369,6 +372,7 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     if (slots * a->kv_heads > (1u << 30)) return fail("attn_prompt_dev: too many rows");
     p.slots = (int)slots;
     p.items = (int)(slots * a->kv_heads);
+    const size_t steps = (keys->rows + AP_ROWS - 1) / AP_ROWS;     /* of a tile, at most */
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
     Ctx *c = g_ctx;
@@ -376,6 +380,18 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     cudaStream_t st = (cudaStream_t)stream;
     Ordered ord(c, st);
     if (ord.rc) return 1;
+    /* Tiles that leave SMs idle share their keys, by four steps of 128 at least: the second kernel
+     * takes as long as two or three.  head_dim 256, 2 key heads: 16 rows over 4096 keys 52 -> 31
+     * us, 128 rows over 30128 331 -> 77, one row over 1000 20 -> 17.  Where the parts would fill the SMs, their way
+     * through memory takes longer than a few steps: 400 rows over 1000 keys 21 -> 26, so only
+     * from sixteen steps on. */
+    size_t splits = (size_t)c->sm_count / p.items;
+    if (splits > steps / 4) splits = steps / 4;
+    if (splits > AP_MAX_SPLITS) splits = AP_MAX_SPLITS;
+    if (steps < 16 && 2 * splits * p.items > (size_t)c->sm_count) splits = 1;
+    p.splits = splits > 1 ? (int)splits : 1;
+    p.items *= p.splits;
+    p.parts = c->d_attn_split;
     p.sched = c->d_attn_sync + AD_SYNC_WORDS;
     p.status = c->d_status;
     if (a->head_dim == 64) return launch_prompt<64>(c, p, keys, k_stride, v_stride, st);

@@ -24,6 +24,10 @@
  * reference within the range of fp32 and BF16 gives the same quotient, and O in tensor memory
  * is then hardly ever scaled again (that takes its columns through registers).
  *
+ * Few rows and many keys (the next part of a prompt behind a long one) would leave most SMs
+ * idle: then several CTAs share a tile's keys, leave their sums in fp32 and a second kernel
+ * adds them up in order.
+ *
  * Bound at head_dim 256 and long prompts: shared memory (Q and K for S, V, and what TMA writes:
  * 2560 cycles for 128 keys) beside 2048 of MMAs and 1024 of exponentials (16 a cycle and SM); at
  * 128 the same at half the size, 1280 beside 1024 and 1024; at 64 the exponentials.
@@ -52,6 +56,9 @@ constexpr int AP_REGS_ISSUE = 40, AP_REGS_SOFT = 232;
 constexpr int AP_TMEM_COLS = 512;
 constexpr int AP_TMEM_O = 256;               /* scores in columns 0..255 */
 constexpr int AP_ITEMS = 2;
+constexpr int AP_MAX_SPLITS = 16;
+/* outputs of 128 rows as they are in tensor memory, then each row's maximum and sum */
+constexpr int AP_PART_FLOATS = AP_ROWS * (256 + 2);
 
 template <int D>
 struct ApShape {
@@ -69,7 +76,9 @@ struct PromptParams {
     const int32_t *cu_q, *cu_k;
     int k_rows, seqs, causal, kv_heads;
     int tile_tokens;                         /* 128 / group */
-    int slots, items;                        /* tiles that there may be, times key heads */
+    int slots, items;                        /* tiles that there may be, times key heads and splits */
+    int splits;                              /* CTAs that share a tile's keys */
+    float *parts;                            /* with splits: their results, [items][AP_PART_FLOATS] */
     unsigned *sched;                         /* next item; [32]: CTAs that are through */
     int *status;
 };
@@ -79,6 +88,7 @@ struct ApItem {
     int head, tiles;                         /* key head, steps of 128 keys */
     int key, keys;                           /* first row of k; keys that the last token sees */
     int sees;                                /* keys that the first token sees */
+    int part;                                /* with splits: whose result it is */
 };
 struct ApShared {
     uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free;
@@ -260,7 +270,7 @@ __device__ __forceinline__ uint64_t ap_desc_mn(uint32_t saddr, uint32_t block_by
 }
 constexpr uint32_t AP_B_MN = 1u << 16;       /* instruction descriptor: B is MN-major */
 
-/* The tile of an index, by a whole warp.  Sequence i's tiles have the slots from
+/* The tile of an index (without splits), by a whole warp.  Sequence i's tiles have the slots from
  * cu_q[i] / tile_tokens + i on: one more than it needs, at most, and no sums over sequences. */
 __device__ __forceinline__ ApItem ap_find(const PromptParams &p, int index) {
     const int lane = threadIdx.x & 31, T = p.tile_tokens;
@@ -290,6 +300,20 @@ __device__ __forceinline__ ApItem ap_find(const PromptParams &p, int index) {
         t.keys = max(0, t.sees + t.tokens - 1);
     }
     t.tiles = (t.keys + AP_ROWS - 1) / AP_ROWS;
+    t.part = 0;
+    return t;
+}
+/* The same where CTAs share a tile: the keys of one of them, as if they were all there are. */
+__device__ __forceinline__ ApItem ap_find_part(const PromptParams &p, int index) {
+    if (p.splits == 1) return ap_find(p, index);
+    ApItem t = ap_find(p, index / p.splits);
+    const int per = (t.tiles + p.splits - 1) / p.splits * AP_ROWS;
+    const int from = (index % p.splits) * per;
+    t.key += from;
+    t.sees -= from;
+    t.keys = min(max(t.keys - from, 0), per);
+    t.tiles = (t.keys + AP_ROWS - 1) / AP_ROWS;
+    t.part = index;
     return t;
 }
 
@@ -393,7 +417,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             ApItem t;
             t.tokens = -1;
             while (index < p.items) {
-                t = ap_find(p, index);
+                t = ap_find_part(p, index);
                 if (t.tokens > 0) break;
                 t.tokens = -1;
                 index = p.items > (int)gridDim.x
@@ -704,7 +728,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 __syncwarp();
             };
-            if (p.a.gate) load_gate(0);
+            if (p.a.gate && p.splits == 1) load_gate(0);
             if (t.tiles) {
                 s.sum[half][row] = sum;
                 if (!exchange()) break;
@@ -713,13 +737,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             const float inv = __fdividef(1.0f, sum);
 #pragma unroll 1
-            for (int i = 0; i < 2 * CHUNKS; i++) {
+            for (int i = 0; i < (p.splits > 1 && !t.tiles ? 0 : 2 * CHUNKS); i++) {
                 uint4 now[2][PIECES];
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int w = 0; w < PIECES; w++) now[k][w] = gate[k][w];
-                if (p.a.gate && i + 1 < 2 * CHUNKS) load_gate(i + 1);
+                if (p.a.gate && p.splits == 1 && i + 1 < 2 * CHUNKS) load_gate(i + 1);
                 uint32_t o[CHUNK / 2];
                 if (t.tiles) {
                     tmem_ld_16x256(tmem + lanes + ((uint32_t)(i / CHUNKS * 16) << 16) + AP_TMEM_O +
@@ -745,6 +769,15 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                             e[x][1] = o[(w * 4 + x) * 4 + k * 2 + 1];
                         }
                         ap_turn(e, t4);
+                        if (p.splits > 1) {               /* as it is, for attn_prompt_join_kernel */
+                            float *to = p.parts + (size_t)t.part * AP_PART_FLOATS +
+                                        (quarter * 32 + from) * D + half * (D / 2) +
+                                        (i % CHUNKS) * CHUNK + t4 * 8 + w * 32;
+                            uint4 *to4 = reinterpret_cast<uint4 *>(to);
+                            to4[0] = make_uint4(e[0][0], e[0][1], e[1][0], e[1][1]);
+                            to4[1] = make_uint4(e[2][0], e[2][1], e[3][0], e[3][1]);
+                            continue;
+                        }
                         uint32_t v[4];
                         const uint32_t z[4] = {now[k][w].x, now[k][w].y, now[k][w].z, now[k][w].w};
 #pragma unroll
@@ -764,7 +797,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 __syncwarp();
             }
-            if (p.a.lse && real && half == 0)
+            if (p.splits > 1 && half == 0)
+                *reinterpret_cast<float2 *>(p.parts + (size_t)t.part * AP_PART_FLOATS +
+                                            AP_ROWS * 256 + row * 2) = make_float2(top, sum);
+            if (p.splits == 1 && p.a.lse && real && half == 0)
                 p.a.lse[r * p.a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
             if (t.tiles) {
                 tc_fence_before();
@@ -780,6 +816,63 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, AP_TMEM_COLS);
+    }
+}
+
+/* Tiles whose keys several CTAs have shared: a warp to a row, the parts in order. */
+template <int D>
+__global__ void __launch_bounds__(256) attn_prompt_join_kernel(const __grid_constant__ PromptParams p) {
+    pdl_enter();
+    constexpr int N = D / 32;                /* values of a lane */
+    const ApItem t = ap_find(p, blockIdx.x);
+    const int lane = threadIdx.x & 31;
+    for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < t.tokens * p.a.group;
+         row += 8 * gridDim.y) {
+        float2 ml[AP_MAX_SPLITS];
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < AP_MAX_SPLITS; k++)
+            if (k < p.splits) {
+                ml[k] = *reinterpret_cast<const float2 *>(
+                    p.parts + (size_t)(blockIdx.x * p.splits + k) * AP_PART_FLOATS +
+                    AP_ROWS * 256 + row * 2);
+                top = fmaxf(top, ml[k].x);
+            }
+        float acc[N] = {};
+#pragma unroll
+        for (int k = 0; k < AP_MAX_SPLITS; k++)
+            if (k < p.splits && ml[k].y != 0.0f) {        /* (a part without keys has no outputs) */
+                const float f = exp2_fast(ml[k].x - top);
+                const float *o = p.parts + (size_t)(blockIdx.x * p.splits + k) * AP_PART_FLOATS +
+                                 row * D + lane * N;
+                sum = fmaf(f, ml[k].y, sum);
+#pragma unroll
+                for (int i = 0; i < N; i += 2) {
+                    const float2 v = *reinterpret_cast<const float2 *>(o + i);
+                    acc[i] = fmaf(f, v.x, acc[i]);
+                    acc[i + 1] = fmaf(f, v.y, acc[i + 1]);
+                }
+            }
+        const int in_tile = row / p.a.group;
+        const long token = t.token + in_tile;
+        const int head = t.head * p.a.group + row - in_tile * p.a.group;
+        const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
+        const int at = head * D + lane * N;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            float a = acc[i] * inv, b = acc[i + 1] * inv;
+            if (p.a.gate) {
+                const uint32_t z = *reinterpret_cast<const uint32_t *>(
+                    p.a.gate + token * p.a.gate_stride + at + i);
+                a *= ad_gate(bf16lo(z));
+                b *= ad_gate(bf16hi(z));
+            }
+            *reinterpret_cast<uint32_t *>(p.a.out + token * p.a.out_stride + at + i) =
+                pack_bf16_rn(a, b);
+        }
+        if (p.a.lse && lane == 0)
+            p.a.lse[token * p.a.heads + head] =
+                sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
     }
 }
 

@@ -134,6 +134,7 @@ struct Ctx {
      * the tile counters of attention over prompts (attn_prompt.cuh) */
     uint2 *d_attn_parts = nullptr;
     unsigned *d_attn_sync = nullptr;
+    float *d_attn_split = nullptr;       /* [sm_count][AP_PART_FLOATS] */
     size_t df_act_elems = 0, df_sa_elems = 0;
     int last_block_launches = 0;
     int last_block_path = 0;
@@ -256,6 +257,8 @@ static int ctx_init() {
                      (size_t)c->sm_count * DF_MARKS * sizeof(unsigned long long)));
     CU_OK(cudaMalloc(&c->d_attn_parts, ad_scratch_bytes(c->sm_count)));
     CU_OK(cudaMemset(c->d_attn_parts, 0, ad_scratch_bytes(c->sm_count)));
+    CU_OK(cudaMalloc(&c->d_attn_split,
+                     (size_t)c->sm_count * AP_PART_FLOATS * sizeof(float)));
     CU_OK(cudaMalloc(&c->d_attn_sync, 2 * AD_SYNC_WORDS * sizeof(unsigned)));
     CU_OK(cudaMemset(c->d_attn_sync, 0, 2 * AD_SYNC_WORDS * sizeof(unsigned)));
     g_apus_use_pdl = env_long("APUS_CUDA_PDL", 1) != 0;
@@ -458,6 +461,7 @@ extern "C" void apus_cuda_disable(void) {
     if (c->d_df_timeline) cudaFree(c->d_df_timeline);
     if (c->d_attn_parts) cudaFree(c->d_attn_parts);
     if (c->d_attn_sync) cudaFree(c->d_attn_sync);
+    if (c->d_attn_split) cudaFree(c->d_attn_split);
     if (c->d_df_act) cudaFree(c->d_df_act);
     if (c->d_df_sa) cudaFree(c->d_df_sa);
     if (c->d_router_logits) cudaFree(c->d_router_logits);

@@ -8,7 +8,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 HEADS = [(16, 2, 256), (32, 8, 128), (20, 4, 128), (12, 12, 64), (16, 1, 128), (6, 2, 64),
-         (3, 3, 256)]
+         (3, 3, 256), (16, 1, 256)]
 
 
 def _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, causal=True, gate=True, pad=0, seed=0,
@@ -66,6 +66,17 @@ def test_prompt_keys_before_and_missing(gpu, nq, nk, heads, kv_heads, dim):
     import torch
     _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, seed=3)
     _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, causal=False, seed=4)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 1, 128), (4, 2, 64),
+                                                (5, 1, 128)])
+@pytest.mark.parametrize("nq,nk", [([1], [5000]), ([20], [4111]), ([3, 9], [2000, 1]),
+                                   ([7, 2], [0, 3001]), ([33], [1024])])
+def test_prompt_few_rows_many_keys(gpu, heads, kv_heads, dim, nq, nk):
+    """Keys shared by several CTAs: parts that see all, some and no keys of theirs."""
+    import torch
+    _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, seed=5)
+    _prompt(gpu, torch, nq, nk, heads, kv_heads, dim, causal=False, gate=False, seed=6, spoil=True)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
