@@ -197,6 +197,9 @@ extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *
         sum += r->sections[a];
     }
     if (sum != pairs) return fail("rope_dev: sections must add up to rot_dim / 2");
+    /* theta^(-2 i / rot_dim) / 2 pi, as products of 64 bits: a last bit of a double at most */
+    const long double ratio = powl((long double)r->theta, -2.0L / (long double)r->rot_dim);
+    long double turns = 1.0L / 6.283185307179586476925286766559L;
     for (size_t i = 0, a = 0, in = 0; i < pairs; i++) {
         if (r->interleaved) {
             a = i % r->axes;
@@ -210,8 +213,8 @@ extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *
         }
         count[a]++;
         p.axis[i] = (unsigned char)a;
-        p.turns[i] = pow(r->theta, -2.0 * (double)i / (double)r->rot_dim) /
-                     6.283185307179586476925286766559;
+        p.turns[i] = (double)turns;
+        turns *= ratio;
     }
     for (size_t a = 0; a < r->axes; a++)
         if (count[a] != r->sections[a])
@@ -256,14 +259,18 @@ extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
     DeviceGuard dev(g_ctx->device);
-    /* tokens to a CTA: as many as give every thread an angle, fewer where that leaves SMs idle */
-    size_t tokens = ROPE_THREADS / pairs ? ROPE_THREADS / pairs : 1;
-    while (tokens > 1 && (r->rows + tokens - 1) / tokens < 2 * (size_t)g_ctx->sm_count)
-        tokens /= 2;
-    p.tokens = (int)tokens;
-    LAUNCH_OK(launch_k(rope_kernel, dim3((unsigned)((r->rows + tokens - 1) / tokens)),
-                       dim3(ROPE_THREADS), tokens * pairs * sizeof(float2), (cudaStream_t)stream,
-                       p));
+    /* warps to a token: as many as its vectors are worth, while there are SMs without any */
+    const size_t vectors = r->heads + r->kv_heads * (kv ? 2 : 1), at_once = 256 / r->head_dim;
+    size_t split = 1;
+    while (2 * split * at_once <= vectors && r->rows * split < 8 * (size_t)g_ctx->sm_count) split *= 2;
+    p.split = (int)split;
+    constexpr size_t warps = ROPE_THREADS / 32;
+    const dim3 grid((unsigned)((r->rows * split + warps - 1) / warps));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (r->head_dim == 64) LAUNCH_OK(launch_k(rope_kernel<64>, grid, dim3(ROPE_THREADS), 0, st, p));
+    else if (r->head_dim == 128)
+        LAUNCH_OK(launch_k(rope_kernel<128>, grid, dim3(ROPE_THREADS), 0, st, p));
+    else LAUNCH_OK(launch_k(rope_kernel<256>, grid, dim3(ROPE_THREADS), 0, st, p));
     return 0;
 }
 
