@@ -33,7 +33,7 @@ static int kv_view(const ApusCudaKvCache *kv, const char *what, KvView *out) {
         return fail("%s: the pools must be 16-byte aligned", what);
     const size_t most = 0x7fffffff;
     if (kv->kv_heads > 1024 || kv->pages > most / (kv->page_tokens * kv->kv_heads) ||
-        kv->max_pages > most / kv->page_tokens || kv->layers > 65536 || kv->seqs > most / 64 ||
+        kv->max_pages > most / kv->page_tokens || kv->layers > 65536 || kv->seqs > (size_t)KV_MAX_SEQS ||
         kv->kv_heads * kv->page_tokens > most / kv->head_dim)
         return fail("%s: the cache is too large", what);
     KvView v;
@@ -159,6 +159,12 @@ extern "C" int apus_cuda_kv_copy_dev(const ApusCudaKvCache *kv, const int32_t *d
     if (ctx_init()) return 1;
     DeviceGuard dev(g_ctx->device);
     cudaStream_t st = (cudaStream_t)stream;
+    if (n <= KV_CHECK_LIST && v.pages <= KV_CHECK_PAGES) {
+        LAUNCH_OK(launch_k(kv_apply_kernel<KV_APPLY_LIST>, dim3(kv_apply_grid(g_ctx)),
+                           dim3(KV_APPLY_THREADS), ((size_t)v.pages + 31) / 32 * 4, st, v, d_src,
+                           d_dst, (int)n));
+        return 0;
+    }
     LAUNCH_OK(launch_k(kv_copy_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS), 0, st, v, d_src,
                        d_dst, (int)n));
     LAUNCH_OK(launch_k(kv_apply_kernel<KV_APPLY_COPY>, dim3(kv_apply_grid(g_ctx)),

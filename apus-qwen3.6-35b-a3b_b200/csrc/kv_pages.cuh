@@ -8,12 +8,13 @@
  * call takes follows from them alone (the lowest free ones, in the order of its list), so a
  * result does not depend on the order in which threads run.
  *
- * A call that has to decide for the whole cache first (extend, fork, compact, copy) does so in
- * one CTA (the "plan"): it checks the list, counts, and finds free pages by one pass over refs.
- * refs is read twice by 32 warps, each over its own piece with eight loads in flight: 4 bytes a
- * page, out of L2 from the second look on.  A plan that cannot be carried out leaves a status and changes nothing.
- * What moves bytes (kv_apply_kernel) runs on all SMs and reads the plan: its bound is HBM, each
- * page read once and written once.
+ * A call that has to decide for the whole cache first (extend, fork, compact) does so in one CTA
+ * (the "plan"): it checks the list, counts, and finds free pages by one look at refs, 4 bytes a
+ * page by 32 warps with eight loads under way each.  What bounds it is the round trips to L2 that
+ * depend on one another (about 0.7 us each), so refs is asked for before the list, and marks of
+ * sequences are bits in shared memory.  A plan that cannot be carried out leaves a status and
+ * changes nothing.  What moves bytes (kv_apply_kernel) runs on all SMs and reads the plan: its
+ * bound is HBM, each page read once and written once (482 MB of pages moved together: 75 us, 6.4 TB/s).
  */
 #pragma once
 #include <cuda_runtime.h>
@@ -30,9 +31,12 @@ constexpr int KV_APPLY_THREADS = 256;
 /* what went wrong first, in work[0] until the caller clears it */
 enum : int { KV_OK = 0, KV_NO_PAGES = 1, KV_BAD_LIST = 2, KV_BAD_PAGE = 3 };
 
+constexpr int KV_MAX_SEQS = 65536;
+constexpr int KV_CHECK_PAGES = 1 << 18, KV_CHECK_LIST = 4096;
+
 /* the caller's scratch: work[0] status, [1] copies, [2] pages in use, [3] plan accepted;
  * from 64 on: copy sources, copy targets, page map, marks of pages; then per entry of a list
- * first fresh page, marks of sequences */
+ * first fresh page, and where a sequence's new tokens start */
 struct KvView {
     uint16_t *k, *v;
     int32_t *refs, *table, *len, *work;
@@ -44,7 +48,7 @@ struct KvView {
     __device__ int32_t *map() const { return work + 64 + 2 * (size_t)pages; }
     __device__ int32_t *mark() const { return work + 64 + 3 * (size_t)pages; }
     __device__ int32_t *first() const { return work + 64 + 4 * (size_t)pages; }
-    __device__ int32_t *seq_mark() const { return first() + seqs; }
+    __device__ int32_t *starts() const { return first() + seqs; }
     /* pages that `tokens` tokens take */
     __device__ int held(int tokens) const {
         return tokens <= 0 ? 0 : min((int)(((unsigned)tokens + page_tokens - 1) / page_tokens),
@@ -80,63 +84,77 @@ __device__ __forceinline__ int kv_block_scan(int v, int *total, int *smem /* [33
     return smem[warp] + x - v;
 }
 
-/* One look at every page by the whole CTA, in ascending order within a warp's piece:
- * f(page, refs != 0, ballot of those in use), called by full warps. */
-template <typename F>
-__device__ __forceinline__ void kv_each_page(const KvView &kv, F f) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int piece = ((kv.pages + 31) / 32 + 255) / 256 * 256;
-    const int lo = min(warp * piece, kv.pages), hi = min(lo + piece, kv.pages);
-    for (int p0 = lo; p0 < hi; p0 += 256) {
-        int r[8];
+/* The pages by the whole CTA, 32 warps with a piece each, in ascending order within it.  The
+ * first 256 of a piece (all of it up to 8192 pages) are asked for when the object is made. */
+struct KvPages {
+    const KvView &kv;
+    int lo, hi, ahead[8];
+    __device__ __forceinline__ explicit KvPages(const KvView &kv_) : kv(kv_) {
+        const int warp = threadIdx.x >> 5;
+        const int piece = ((kv.pages + 31) / 32 + 255) / 256 * 256;
+        lo = min(warp * piece, kv.pages);
+        hi = min(lo + piece, kv.pages);
+        load(lo, ahead);
+    }
+    __device__ __forceinline__ void load(int p0, int (&r)[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int p = p0 + i * 32 + lane;
+            const int p = p0 + i * 32 + (threadIdx.x & 31);
             r[i] = p < hi ? kv.refs[p] : 0;
         }
+    }
+    /* f(page, whether it is one, whether it is in use), by full warps */
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int p0 = lo; p0 < hi; p0 += 256) {
+            int r[8];
+            if (p0 == lo) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int p = p0 + i * 32 + lane;
-            const unsigned used = __ballot_sync(0xffffffffu, p < hi && r[i] != 0);
-            const unsigned there = __ballot_sync(0xffffffffu, p < hi);
-            f(p, p < hi, r[i] != 0, used, there);
+                for (int i = 0; i < 8; i++) r[i] = ahead[i];
+            } else {
+                load(p0, r);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int p = p0 + i * 32 + (threadIdx.x & 31);
+                f(p, p < hi, r[i] != 0);
+            }
         }
     }
-}
-
-/* The first `want` free pages in ascending order into list; how many are free.  (All threads.) */
-__device__ __forceinline__ int kv_find_free(const KvView &kv, int want, int32_t *list,
-                                            int *smem) {
-    const int lane = threadIdx.x & 31;
-    int mine = 0;
-    kv_each_page(kv, [&](int, bool, bool, unsigned used, unsigned there) {
-        mine += __popc(there & ~used);
-    });
-    int total;
-    int at = kv_block_scan(lane == 0 ? mine : 0, &total, smem);
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (total >= want)
-        kv_each_page(kv, [&](int p, bool there, bool used, unsigned u, unsigned t) {
-            const unsigned freed = t & ~u;
-            const int r = at + __popc(freed & ((1u << lane) - 1));
-            if (there && !used && r < want) list[r] = p;
-            at += __popc(freed);
+    /* The first `want` free pages in ascending order into list; how many are free. */
+    __device__ __forceinline__ int find_free(int want, int32_t *list, int *smem) const {
+        const int lane = threadIdx.x & 31;
+        int mine = 0;
+        each([&](int, bool there, bool used) {
+            mine += __popc(__ballot_sync(0xffffffffu, there && !used));
         });
-    __syncthreads();
-    return total;
-}
+        int total;
+        int at = kv_block_scan(lane == 0 ? mine : 0, &total, smem);
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (total >= want)
+            each([&](int p, bool there, bool used) {
+                const unsigned freed = __ballot_sync(0xffffffffu, there && !used);
+                const int r = at + __popc(freed & ((1u << lane) - 1));
+                if (there && !used && r < want) list[r] = p;
+                at += __popc(freed);
+            });
+        __syncthreads();
+        return total;
+    }
+};
 
-/* Sequences of a list: in range, none twice.  (All threads; true where the list is sound.) */
-__device__ __forceinline__ bool kv_check_list(const KvView &kv, const int32_t *seq, int n) {
+/* Sequences of a list: in range, none twice; their bits are set then.  (All threads; true where
+ * the list is sound.) */
+__device__ __forceinline__ bool kv_check_list(const KvView &kv, const int32_t *seq, int n,
+                                              unsigned *bits /* [KV_MAX_SEQS / 32] */) {
+    for (int i = threadIdx.x; i < (kv.seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
+    __syncthreads();
     int bad = 0;
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const int s = seq ? seq[i] : i;
-        if (s < 0 || s >= kv.seqs) bad = 1;
-        else kv.seq_mark()[s] = 0;
+        if ((unsigned)s >= (unsigned)kv.seqs) bad = 1;
+        else if (atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad = 1;
     }
-    if (__syncthreads_or(bad)) return false;
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-        if (atomicAdd(&kv.seq_mark()[seq ? seq[i] : i], 1)) bad = 1;
     return !__syncthreads_or(bad);
 }
 
@@ -147,8 +165,10 @@ kv_extend_kernel(KvView kv, const int32_t *__restrict__ seq, const int32_t *__re
                  int32_t *__restrict__ slot, int rows) {
     pdl_enter();
     __shared__ int smem[33];
+    __shared__ unsigned bits[KV_MAX_SEQS / 32];
     const int tid = threadIdx.x;
-    int code = kv_check_list(kv, seq, n) ? KV_OK : KV_BAD_LIST;
+    const KvPages pages(kv);
+    int code = kv_check_list(kv, seq, n, bits) ? KV_OK : KV_BAD_LIST;
     int taken = 0;
     if (code == KV_OK) {
         int bad = 0;
@@ -169,7 +189,7 @@ kv_extend_kernel(KvView kv, const int32_t *__restrict__ seq, const int32_t *__re
         if (__syncthreads_or(bad)) code = KV_BAD_LIST;
     }
     if (code == KV_OK && taken > 0) {
-        if (taken > kv.pages || kv_find_free(kv, taken, kv.copy_src(), smem) < taken)
+        if (taken > kv.pages || pages.find_free(taken, kv.copy_src(), smem) < taken)
             code = KV_NO_PAGES;
     }
     if (code != KV_OK) {
@@ -187,7 +207,7 @@ kv_extend_kernel(KvView kv, const int32_t *__restrict__ seq, const int32_t *__re
             kv.table[(size_t)s * kv.max_pages + j] = p;
             kv.refs[p] = 1;
         }
-        if ((tid & 31) == 0) kv.seq_mark()[s] = old;      /* where the new tokens start */
+        if ((tid & 31) == 0) kv.starts()[s] = old;
         __syncwarp();
         if ((tid & 31) == 0) kv.len[s] = now;
     }
@@ -202,7 +222,7 @@ kv_extend_kernel(KvView kv, const int32_t *__restrict__ seq, const int32_t *__re
         }
         int where = -1;
         if (lo < n && t >= cu[lo]) {
-            const int s = seq ? seq[lo] : lo, at = kv.seq_mark()[s] + t - cu[lo];
+            const int s = seq ? seq[lo] : lo, at = kv.starts()[s] + t - cu[lo];
             const int p = kv.table[(size_t)s * kv.max_pages + at / kv.page_tokens];
             if ((unsigned)p < (unsigned)kv.pages) where = p * kv.page_tokens + at % kv.page_tokens;
             else atomicCAS(kv.status(), 0, KV_BAD_PAGE);
@@ -247,40 +267,36 @@ kv_fork_plan_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *_
                     int n) {
     pdl_enter();
     __shared__ int smem[33];
+    __shared__ unsigned bits[KV_MAX_SEQS / 32];
     const int tid = threadIdx.x;
-    int code = kv_check_list(kv, dst, n) ? KV_OK : KV_BAD_LIST, taken = 0;
+    const KvPages pages(kv);
+    int code = kv_check_list(kv, dst, n, bits) ? KV_OK : KV_BAD_LIST, taken = 0;
     int bad = 0;
-    if (code == KV_OK) {
-        for (int i = tid; i < n; i += KV_PLAN_THREADS) {
-            const int s = src[i];
-            if (s < 0 || s >= kv.seqs) bad = 1;
-            else if (kv.len[s] < 0 || kv.len[dst[i]] != 0) bad = 1;
-        }
-        if (__syncthreads_or(bad)) code = KV_BAD_LIST;
-    }
-    if (code == KV_OK) {
-        /* none is written that another one is read from: marks of the written ones are all 1 */
-        for (int i = tid; i < n; i += KV_PLAN_THREADS) kv.seq_mark()[src[i]] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += KV_PLAN_THREADS) kv.seq_mark()[dst[i]] = 1;
-        __syncthreads();
-        for (int i = tid; i < n; i += KV_PLAN_THREADS)
-            if (kv.seq_mark()[src[i]]) bad = 1;
-        if (__syncthreads_or(bad)) code = KV_BAD_LIST;
-    }
     if (code == KV_OK) {
         for (int i0 = 0; i0 < n; i0 += KV_PLAN_THREADS) {
             const int i = i0 + tid;
-            const int need = i < n && kv.len[src[i]] % kv.page_tokens ? 1 : 0;
+            int need = 0;
+            if (i < n) {
+                const int s = src[i];
+                /* (none is written that another one is read from) */
+                if ((unsigned)s >= (unsigned)kv.seqs || (bits[s >> 5] >> (s & 31) & 1)) {
+                    bad = 1;
+                } else {
+                    const int tokens = kv.len[s];
+                    if (tokens < 0 || kv.len[dst[i]] != 0) bad = 1;
+                    else need = tokens % kv.page_tokens ? 1 : 0;
+                }
+            }
             int total;
             const int at = kv_block_scan(need, &total, smem);
             if (i < n) kv.first()[i] = taken + at;
             taken += total;
         }
-        __syncthreads();
-        if (taken && (taken > kv.pages || kv_find_free(kv, taken, kv.copy_dst(), smem) < taken))
-            code = KV_NO_PAGES;
+        if (__syncthreads_or(bad)) code = KV_BAD_LIST;
     }
+    if (code == KV_OK && taken &&
+        (taken > kv.pages || pages.find_free(taken, kv.copy_dst(), smem) < taken))
+        code = KV_NO_PAGES;
     if (code == KV_OK) {
         for (int i = tid; i < n; i += KV_PLAN_THREADS) {
             const int tokens = kv.len[src[i]];
@@ -307,11 +323,14 @@ kv_compact_plan_kernel(KvView kv) {
     pdl_enter();
     __shared__ int smem[33];
     const int lane = threadIdx.x & 31;
+    const KvPages pages(kv);
     int mine = 0, live;
-    kv_each_page(kv, [&](int, bool, bool, unsigned used, unsigned) { mine += __popc(used); });
+    pages.each([&](int, bool there, bool used) {
+        mine += __popc(__ballot_sync(0xffffffffu, there && used));
+    });
     kv_block_scan(lane == 0 ? mine : 0, &live, smem);
     int leave = 0, fill = 0;
-    kv_each_page(kv, [&](int p, bool there, bool used, unsigned, unsigned) {
+    pages.each([&](int p, bool there, bool used) {
         leave += __popc(__ballot_sync(0xffffffffu, there && used && p >= live));
         fill += __popc(__ballot_sync(0xffffffffu, there && !used && p < live));
     });
@@ -320,7 +339,7 @@ kv_compact_plan_kernel(KvView kv) {
     int at_fill = kv_block_scan(lane == 0 ? fill : 0, &same, smem);
     at_leave = __shfl_sync(0xffffffffu, at_leave, 0);
     at_fill = __shfl_sync(0xffffffffu, at_fill, 0);
-    kv_each_page(kv, [&](int p, bool there, bool used, unsigned, unsigned) {
+    pages.each([&](int p, bool there, bool used) {
         const unsigned below = (1u << lane) - 1;
         const bool l = there && used && p >= live, f = there && !used && p < live;
         const unsigned bl = __ballot_sync(0xffffffffu, l), bf = __ballot_sync(0xffffffffu, f);
@@ -343,7 +362,8 @@ kv_compact_plan_kernel(KvView kv) {
     }
 }
 
-/* A list of pages as it came: in range, no target twice or a source as well. */
+/* A list of pages as it came: in range, no target twice or a source as well.  (Long lists and large
+ * pools; else every CTA that copies looks for itself.) */
 __global__ void __launch_bounds__(KV_PLAN_THREADS)
 kv_copy_plan_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
                     int n) {
@@ -378,14 +398,41 @@ kv_copy_plan_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *_
 
 /* The plan carried out: tables (fork: a CTA to an entry of the list; compact: a warp to a
  * sequence), then the copies, 16 KB of a page at a time. */
-enum : int { KV_APPLY_COPY = 0, KV_APPLY_FORK = 1, KV_APPLY_COMPACT = 2 };
+enum : int { KV_APPLY_COPY = 0, KV_APPLY_FORK = 1, KV_APPLY_COMPACT = 2, KV_APPLY_LIST = 3 };
 template <int WHAT>
 __global__ void __launch_bounds__(KV_APPLY_THREADS)
 kv_apply_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
                 int n) {
     pdl_enter();
     const int tid = threadIdx.x;
-    if (!kv.work[3]) return;
+    extern __shared__ unsigned kv_bits[];
+    if (WHAT == KV_APPLY_LIST) {
+        /* the list as it came, checked by every CTA with a bit for each page: one launch less */
+        for (int i = tid; i < (kv.pages + 31) / 32; i += KV_APPLY_THREADS) kv_bits[i] = 0;
+        __syncthreads();
+        int code = KV_OK;
+        for (int i = tid; i < n; i += KV_APPLY_THREADS) {
+            const unsigned s = src[i], d = dst[i];
+            if (s >= (unsigned)kv.pages || d >= (unsigned)kv.pages) code = KV_BAD_PAGE;
+            else if (atomicOr(&kv_bits[d >> 5], 1u << (d & 31)) >> (d & 31) & 1)
+                code = KV_BAD_LIST;
+        }
+        __syncthreads();
+        for (int i = tid; i < n; i += KV_APPLY_THREADS) {
+            const unsigned s = src[i];
+            if (s < (unsigned)kv.pages && (kv_bits[s >> 5] >> (s & 31) & 1) && code == KV_OK)
+                code = KV_BAD_LIST;
+        }
+        const bool page = __syncthreads_or(code == KV_BAD_PAGE),
+                   list = __syncthreads_or(code == KV_BAD_LIST);
+        if (page || list) {
+            if (blockIdx.x == 0 && tid == 0)
+                atomicCAS(kv.status(), 0, page ? KV_BAD_PAGE : KV_BAD_LIST);
+            return;
+        }
+    } else if (!kv.work[3]) {
+        return;
+    }
     if (WHAT == KV_APPLY_FORK) {
         for (int i = blockIdx.x; i < n; i += gridDim.x) {
             const int s = src[i], d = dst[i], tokens = kv.len[s];
@@ -417,7 +464,9 @@ kv_apply_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *__res
             }
         }
     }
-    const int copies = kv.work[1];
+    const int copies = WHAT == KV_APPLY_LIST ? n : kv.work[1];
+    const int32_t *from_page = WHAT == KV_APPLY_LIST ? src : kv.copy_src(),
+                  *to_page = WHAT == KV_APPLY_LIST ? dst : kv.copy_dst();
     const int page16 = kv.page_elems / 8;                 /* 16-byte pieces of a page */
     constexpr int UNIT = 4 * KV_APPLY_THREADS;            /* of which a CTA takes these at a time */
     const int units = (page16 + UNIT - 1) / UNIT;
@@ -430,8 +479,8 @@ kv_apply_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *__res
         const int layer = (int)(r % kv.layers), i = (int)(r / kv.layers);
         const size_t base = (size_t)layer * kv.pages;
         const uint4 *from =
-            reinterpret_cast<const uint4 *>(pool + (base + kv.copy_src()[i]) * kv.page_elems);
-        uint4 *to = reinterpret_cast<uint4 *>(pool + (base + kv.copy_dst()[i]) * kv.page_elems);
+            reinterpret_cast<const uint4 *>(pool + (base + from_page[i]) * kv.page_elems);
+        uint4 *to = reinterpret_cast<uint4 *>(pool + (base + to_page[i]) * kv.page_elems);
         uint4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {

@@ -567,7 +567,8 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  * of k and of v.  Token t of sequence s is token t % page_tokens of page
  * table[s * max_pages + t / page_tokens].  refs counts the sequences that hold a page, 0 is a
  * free one.  A new cache has refs 0, len 0, table -1 and work 0 (k and v as they are).  Entries of the table behind a
- * sequence's last page are not read.  pages * kv_heads * page_tokens < 2^31.
+ * sequence's last page are not read.  pages * kv_heads * page_tokens < 2^31,
+ * seqs at most 65536.
  *
  * work is scratch of the calls on this cache; its first word is the cache's status, which
  * stays at the first thing that went wrong until the caller clears it: 0 ok, 1 pages ran

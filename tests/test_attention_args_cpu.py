@@ -42,7 +42,7 @@ def rope(B, **kw):
 
 BAD_CACHE = [dict(k=None), dict(work=None), dict(pages=0), dict(page_tokens=0),
              dict(page_tokens=24), dict(page_tokens=512), dict(head_dim=96), dict(k=BIG + 8),
-             dict(pages=1 << 28), dict(seqs=0), dict(max_pages=1 << 28)]
+             dict(pages=1 << 28), dict(seqs=0), dict(seqs=65537), dict(max_pages=1 << 28)]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHE)

@@ -206,21 +206,32 @@ def test_lists_that_are_refused_change_nothing(gpu):
     assert int(cache.refs.sum()) == 4
 
 
-def test_copy(gpu):
+@pytest.mark.parametrize("pages,n,layers,kv_heads,page,dim", [
+    (400, 190, 3, 2, 32, 128), (12000, 4500, 1, 1, 16, 64), (300000, 40, 1, 1, 16, 64),
+    (20, 1, 2, 1, 256, 256)])
+def test_copy(gpu, pages, n, layers, kv_heads, page, dim):
+    """Short and long lists, small and large pools; a source may go to several pages."""
     import torch
     import attn_util as u
-    cache = u.Cache(3, 400, 2, 32, 128, 2, 4)
+    cache = u.Cache(layers, pages, kv_heads, page, dim, 2, 4)
     want_k, want_v = cache.k.clone(), cache.v.clone()
-    g = torch.Generator().manual_seed(1)
-    order = torch.randperm(400, generator=g).int().cuda()
-    src = torch.cat([order[:150], order[:40]]).contiguous()     # a source may go to several
-    dst = order[200:390].contiguous()
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).int().cuda()
+    src = torch.cat([order[:n // 2], order[:n - n // 2]]).contiguous()
+    dst = order[n:2 * n].contiguous()
     want_k[:, dst.long()] = want_k[:, src.long()]
     want_v[:, dst.long()] = want_v[:, src.long()]
-    gpu.kv_copy_dev(cache.c, src.data_ptr(), dst.data_ptr(), 190, stream=u.stream())
+    gpu.kv_copy_dev(cache.c, src.data_ptr(), dst.data_ptr(), n, stream=u.stream())
     torch.cuda.synchronize()
     assert cache.status() == 0
     assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)
+    if n > 4:
+        for bad, code in ((dst.clone(), 2), (src.clone(), 2), (dst.clone(), 3)):
+            bad[n - 1] = dst[0] if code == 2 else pages
+            gpu.kv_copy_dev(cache.c, src.data_ptr(), bad.data_ptr(), n, stream=u.stream())
+            torch.cuda.synchronize()
+            assert cache.status() == code
+            cache.work[0] = 0
+            assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)
 
 
 def _rope(gpu, torch, T, heads, kv_heads, dim, rot, axes, interleaved, cache=True, in_place=False,
