@@ -429,7 +429,7 @@ static int decode_map(CUtensorMap *m, const uint16_t *base, size_t rows, size_t 
 template <int D, int NH>
 static int launch_decode(Ctx *c, const CUtensorMap &mk, const CUtensorMap &mv, DecodeParams p,
                          cudaStream_t st) {
-    const int smem = ad_smem_bytes(), grid = c->sm_count < AD_MAX_CTAS ? c->sm_count : AD_MAX_CTAS;
+    const int smem = ad_smem_bytes();
     static bool set = false;
     if (!set) {
         CU_OK(cudaFuncSetAttribute(attn_decode_kernel<D, NH>,
@@ -439,8 +439,12 @@ static int launch_decode(Ctx *c, const CUtensorMap &mk, const CUtensorMap &mv, D
     for (int row = 0; row < p.a.rows; row += AD_MAX_ROWS) {
         p.row0 = row;
         p.rows = p.a.rows - row < AD_MAX_ROWS ? p.a.rows - row : AD_MAX_ROWS;
-        LAUNCH_OK(launch_coop_k(attn_decode_kernel<D, NH>, dim3(grid), dim3(AD_THREADS), smem, st,
-                                mk, mv, p));
+        /* no more CTAs than have a tile for each warp, were all sequences as long as they may be */
+        const size_t tiles = (size_t)p.rows * p.kv_heads * p.max_pages * p.page_tiles;
+        size_t grid = (tiles + AD_WARPS - 1) / AD_WARPS;
+        if (grid > (size_t)c->sm_count) grid = c->sm_count;
+        LAUNCH_OK(launch_coop_k(attn_decode_kernel<D, NH>, dim3((unsigned)grid), dim3(AD_THREADS), smem,
+                                st, mk, mv, p));
     }
     return 0;
 }

@@ -40,7 +40,6 @@ constexpr int AD_THREADS = AD_WARPS * 32;
 constexpr int AD_TILE = 16;                  /* tokens */
 constexpr int AD_MAX_ROWS = 1024;            /* of a launch */
 constexpr int AD_RING_BYTES = 24 << 10;      /* of a warp */
-constexpr int AD_MAX_CTAS = 256;
 constexpr int AD_SYNC_ROUND = 0, AD_SYNC_SEEN = 32, AD_SYNC_WORDS = 64;
 constexpr int AD_MAX_GROUP = 16;
 constexpr int AD_MAX_DIM = 256;
@@ -88,7 +87,8 @@ struct AdShared {
     long long scan[AD_WARPS];
     float weight[2 * AD_WARPS][AD_MAX_GROUP], top[2 * AD_WARPS][AD_MAX_GROUP],
         sum[2 * AD_WARPS][AD_MAX_GROUP];
-    int leads[2 * AD_WARPS], joint[2];
+    unsigned same[2 * AD_WARPS];
+    int leader[2 * AD_WARPS], leaders, joint[2];
 };
 inline int ad_smem_bytes() { return AD_WARPS * AD_RING_BYTES + (int)sizeof(AdShared) + 1024; }
 
@@ -600,65 +600,65 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     __syncthreads();
 
     /* ---- the SM's unfinished results, put together in the order of the line ---- */
+    /* (Loops over the set bits of an entry's mask, not unrolled: what runs once or twice is bound
+     * by its instructions' way out of L2.) */
     constexpr int ENTRIES = 2 * AD_WARPS;
+    static_assert(ENTRIES == 16, "entries are lanes and bits");
+    if (tid < ENTRIES) {
+        const int item = s.item[tid >> 1][tid & 1];
+        const unsigned same = __match_any_sync(0xffffu, item);        /* entries of the same item */
+        const bool leads = item >= 0 && __ffs(same) - 1 == tid;
+        const unsigned leaders = __ballot_sync(0xffffu, leads);
+        s.same[tid] = same;
+        if (leads) s.leader[__popc(leaders & ((1u << tid) - 1))] = tid;
+        if (tid == 0) s.leaders = __popc(leaders);
+    }
+    __syncthreads();
+    const int items = s.leaders;
     {                                                     /* the weight of an entry's head */
         const int e = tid / AD_MAX_GROUP, h = tid % AD_MAX_GROUP;
-        const int item = s.item[e >> 1][e & 1];
-        float top = -INFINITY, sum = 0.0f;
-        bool leads = item >= 0;
-        if (item >= 0 && h < group) {
-#pragma unroll
-            for (int j = 0; j < ENTRIES; j++)
-                if (s.item[j >> 1][j & 1] == item) top = fmaxf(top, s.m[j >> 1][j & 1][h]);
+        if (s.item[e >> 1][e & 1] >= 0 && h < group) {
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+            for (unsigned b = s.same[e]; b; b &= b - 1) {
+                const int j = __ffs(b) - 1;
+                top = fmaxf(top, s.m[j >> 1][j & 1][h]);
+            }
             if (top == -INFINITY) top = 0.0f;             /* nothing counted: weights of 0 */
-#pragma unroll
-            for (int j = 0; j < ENTRIES; j++)
-                if (s.item[j >> 1][j & 1] == item) {
-                    sum = fmaf(exp2_fast(s.m[j >> 1][j & 1][h] - top), s.l[j >> 1][j & 1][h], sum);
-                    if (j < e) leads = false;
-                }
+#pragma unroll 1
+            for (unsigned b = s.same[e]; b; b &= b - 1) {
+                const int j = __ffs(b) - 1;
+                sum = fmaf(exp2_fast(s.m[j >> 1][j & 1][h] - top), s.l[j >> 1][j & 1][h], sum);
+            }
             s.weight[e][h] = exp2_fast(s.m[e >> 1][e & 1][h] - top);
             s.top[e][h] = top;
             s.sum[e][h] = sum;
         }
-        if (h == 0) s.leads[e] = leads;
     }
     __syncthreads();
     constexpr int HEAD4 = D / 4;                          /* pieces of 16 bytes of a head */
     const int per_item = group * HEAD4;
-    int items = 0;
-#pragma unroll
-    for (int e = 0; e < ENTRIES; e++) items += s.leads[e];
 #pragma unroll 1
     for (int x = tid; x < items * per_item; x += AD_THREADS) {
-        int e = -1, nth = x / per_item;
-        const int in = x - nth * per_item, h = in / HEAD4, c = (in - h * HEAD4) * 4;
-        do
-            nth -= s.leads[++e];
-        while (nth >= 0);
-        const int item = s.item[e >> 1][e & 1];
-        float4 v[ENTRIES];
-        float f[ENTRIES];
-#pragma unroll
-        for (int j = 0; j < ENTRIES; j++) {
-            const int w = j >> 1;
-            const bool of = s.item[w][j & 1] == item;
-            const int from_at = h * (D + AD_PAD) + c;
-            f[j] = of ? s.weight[j][h] : 0.0f;
-            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (of)
-                v[j] = j & 1 ? *reinterpret_cast<const float4 *>(
-                                   ring0 + w * AD_RING_BYTES + from_at * 4)
-                             : *reinterpret_cast<const float4 *>(
-                                   p.parts + (size_t)(blockIdx.x * AD_WARPS + w) * AD_PART_FLOATS + from_at);
-        }
+        const int nth = x / per_item, in = x - nth * per_item;
+        const int h = in / HEAD4, c = (in - h * HEAD4) * 4;
+        const int e = s.leader[nth], item = s.item[e >> 1][e & 1];
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < ENTRIES; j++) {
-            acc.x = fmaf(f[j], v[j].x, acc.x);
-            acc.y = fmaf(f[j], v[j].y, acc.y);
-            acc.z = fmaf(f[j], v[j].z, acc.z);
-            acc.w = fmaf(f[j], v[j].w, acc.w);
+#pragma unroll 1
+        for (unsigned b = s.same[e]; b; b &= b - 1) {
+            const int j = __ffs(b) - 1, w = j >> 1;
+            const float f = s.weight[j][h];
+            const int from_at = h * (D + AD_PAD) + c;
+            const float4 v = j & 1
+                                 ? *reinterpret_cast<const float4 *>(ring0 + w * AD_RING_BYTES +
+                                                                     from_at * 4)
+                                 : *reinterpret_cast<const float4 *>(
+                                       p.parts + (size_t)(blockIdx.x * AD_WARPS + w) *
+                                                     AD_PART_FLOATS + from_at);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
         }
         const AdItem it(s, item, p.kv_heads, lo, hi);
         const float top = s.top[e][h], sum = s.sum[e][h];
@@ -675,8 +675,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     /* ---- items that several SMs hold parts of ---- */
     if (tid < 2) s.joint[tid] = -1;
     __syncthreads();
-    if (tid < ENTRIES && s.leads[tid]) {
-        const int item = s.item[tid >> 1][tid & 1];
+    if (tid < items) {
+        const int e = s.leader[tid], item = s.item[e >> 1][e & 1];
         const AdItem it(s, item, p.kv_heads, lo, hi);
         if (it.before || it.after) s.joint[!it.before] = item;
     }
