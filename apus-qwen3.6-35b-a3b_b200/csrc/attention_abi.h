@@ -344,16 +344,19 @@ static int launch_prompt(Ctx *c, const PromptParams &p, const ApusCudaAttnKeys *
     constexpr int smem = ap_smem_bytes<D>();
     static bool set = false;
     if (!set) {
-        CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+        CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D, false>, attr, smem));
+        CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D, true>, attr, smem));
         set = true;
     }
-    const int grid = p.items < c->sm_count ? p.items : c->sm_count;
-    LAUNCH_OK(launch_k(attn_prompt_kernel<D>, dim3(grid), dim3(AP_THREADS), smem, st, mq, mk, mv,
+    const dim3 grid(p.items < c->sm_count ? p.items : c->sm_count), block(AP_THREADS);
+    if (p.splits == 1) {
+        LAUNCH_OK(launch_k(attn_prompt_kernel<D, false>, grid, block, smem, st, mq, mk, mv, p));
+        return 0;
+    }
+    LAUNCH_OK(launch_k(attn_prompt_kernel<D, true>, grid, block, smem, st, mq, mk, mv, p));
+    LAUNCH_OK(launch_k(attn_prompt_join_kernel<D>, dim3(p.items / p.splits, 4), dim3(256), 0, st,
                        p));
-    if (p.splits > 1)
-        LAUNCH_OK(launch_k(attn_prompt_join_kernel<D>, dim3(p.items / p.splits, 4), dim3(256), 0,
-                           st, p));
     return 0;
 }
 

@@ -469,10 +469,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             f[n] = 1.0f;
             if (x > m[n] + 8.0f || (m[n] == -INFINITY && x > -INFINITY)) {
+                moved |= m[n] > -INFINITY;               /* (else there is nothing to scale) */
                 f[n] = exp2_fast(m[n] - x);
                 m[n] = x;
                 l[n] *= f[n];
-                moved = true;
             }
         }
         if (__any_sync(0xffffffffu, moved)) {

@@ -305,7 +305,6 @@ __device__ __forceinline__ ApItem ap_find(const PromptParams &p, int index) {
 }
 /* The same where CTAs share a tile: the keys of one of them, as if they were all there are. */
 __device__ __forceinline__ ApItem ap_find_part(const PromptParams &p, int index) {
-    if (p.splits == 1) return ap_find(p, index);
     ApItem t = ap_find(p, index / p.splits);
     const int per = (t.tiles + p.splits - 1) / p.splits * AP_ROWS;
     const int from = (index % p.splits) * per;
@@ -317,7 +316,8 @@ __device__ __forceinline__ ApItem ap_find_part(const PromptParams &p, int index)
     return t;
 }
 
-template <int D>
+/* SPLIT: CTAs share the keys of a tile, and what a tile ends with is left as it is. */
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(AP_THREADS, 1)
 attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k,
@@ -417,7 +417,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             ApItem t;
             t.tokens = -1;
             while (index < p.items) {
-                t = ap_find_part(p, index);
+                t = SPLIT ? ap_find_part(p, index) : ap_find(p, index);
                 if (t.tokens > 0) break;
                 t.tokens = -1;
                 index = p.items > (int)gridDim.x
@@ -612,7 +612,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             const bool real = my_token < t.tokens;
             const long r = t.token + my_token;
             const int h = t.head * p.a.group + my_head;
-            if (p.a.gate && real)                         /* to L2, for the end of the tile */
+            if (!SPLIT && p.a.gate && real)               /* to L2, for the end of the tile */
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 64)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(
@@ -728,7 +728,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 __syncwarp();
             };
-            if (p.a.gate && p.splits == 1) load_gate(0);
+            if (p.a.gate && !SPLIT) load_gate(0);
             if (t.tiles) {
                 s.sum[half][row] = sum;
                 if (!exchange()) break;
@@ -737,13 +737,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             const float inv = __fdividef(1.0f, sum);
 #pragma unroll 1
-            for (int i = 0; i < (p.splits > 1 && !t.tiles ? 0 : 2 * CHUNKS); i++) {
+            for (int i = 0; i < (SPLIT && !t.tiles ? 0 : 2 * CHUNKS); i++) {
                 uint4 now[2][PIECES];
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int w = 0; w < PIECES; w++) now[k][w] = gate[k][w];
-                if (p.a.gate && p.splits == 1 && i + 1 < 2 * CHUNKS) load_gate(i + 1);
+                if (p.a.gate && !SPLIT && i + 1 < 2 * CHUNKS) load_gate(i + 1);
                 uint32_t o[CHUNK / 2];
                 if (t.tiles) {
                     tmem_ld_16x256(tmem + lanes + ((uint32_t)(i / CHUNKS * 16) << 16) + AP_TMEM_O +
@@ -769,7 +769,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                             e[x][1] = o[(w * 4 + x) * 4 + k * 2 + 1];
                         }
                         ap_turn(e, t4);
-                        if (p.splits > 1) {               /* as it is, for attn_prompt_join_kernel */
+                        if (SPLIT) {                      /* as it is, for attn_prompt_join_kernel */
                             float *to = p.parts + (size_t)t.part * AP_PART_FLOATS +
                                         (quarter * 32 + from) * D + half * (D / 2) +
                                         (i % CHUNKS) * CHUNK + t4 * 8 + w * 32;
@@ -797,10 +797,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 __syncwarp();
             }
-            if (p.splits > 1 && half == 0)
+            if (SPLIT && half == 0)
                 *reinterpret_cast<float2 *>(p.parts + (size_t)t.part * AP_PART_FLOATS +
                                             AP_ROWS * 256 + row * 2) = make_float2(top, sum);
-            if (p.splits == 1 && p.a.lse && real && half == 0)
+            if (!SPLIT && p.a.lse && real && half == 0)
                 p.a.lse[r * p.a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
             if (t.tiles) {
                 tc_fence_before();
