@@ -347,6 +347,13 @@ static int launch_prompt(Ctx *c, const PromptParams &p, const ApusCudaAttnKeys *
         const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
         CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D, false>, attr, smem));
         CU_OK(cudaFuncSetAttribute(attn_prompt_kernel<D, true>, attr, smem));
+        cudaFuncAttributes one, two;
+        CU_OK(cudaFuncGetAttributes(&one, attn_prompt_kernel<D, false>));
+        CU_OK(cudaFuncGetAttributes(&two, attn_prompt_kernel<D, true>));
+        const int regs = one.numRegs < two.numRegs ? one.numRegs : two.numRegs;
+        if (128 * AP_REGS_ISSUE + (AP_THREADS - 128) * AP_REGS_SOFT > AP_THREADS * regs)
+            return fail("attn_prompt_dev: built with %d registers a thread, fewer than its warps "
+                        "hand over", regs);
         set = true;
     }
     const dim3 grid(p.items < c->sm_count ? p.items : c->sm_count), block(AP_THREADS);

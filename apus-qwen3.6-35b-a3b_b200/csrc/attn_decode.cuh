@@ -681,6 +681,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
         if (it.before || it.after) s.joint[!it.before] = item;
     }
     __syncthreads();
+    bool gone = false;                                    /* a part that never came: ask for no other */
 #pragma unroll 1
     for (int j = 0; j < 2; j++) {
         const int item = s.joint[j];
@@ -703,12 +704,13 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             float top = -INFINITY, sum = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-            for (int e = sub; e < n; e += lanes) {
+            for (int e = sub; e < n && !gone; e += lanes) {
                 const uint2 *part =
                     p.shared_parts + (size_t)((c0 + e) * 2 + (e == 0)) * AD_SHARED_WORDS;
                 uint4 a, b, ml;
                 if (!ad_get(part + h * D + c, part + AD_SHARED_ML + 2 * h, round, a, b, ml)) {
                     set_status(p.wait_status, ST_SCHED_TIMEOUT);
+                    gone = true;
                     break;
                 }
                 ad_merge(top, sum, acc, __uint_as_float(ml.x), __uint_as_float(ml.z),

@@ -10,15 +10,17 @@
  *
  * One persistent CTA per SM takes such tiles from a counter (the last tiles of each sequence
  * first: they see the most keys).  Its warps:
- *   warp 0     finds the tile's sequence, loads Q (64 KB at head_dim 256) and a ring of 32 KB pieces of K and V
+ *   warp 0     finds the tile's sequence, loads Q (64 KB at head_dim 256) and a ring of 32 KB
+ *              pieces of K and V
  *   warp 1     issues tcgen05.mma: S(j+1) before O += P(j) V(j), so that the tensor cores work
  *              while the softmax of a step of 128 keys runs
  *   warps 4-11 softmax, two warps to each quarter of the rows with half of the 128 scores each;
  *              outputs at the end
- * S is double-buffered in tensor memory (2 x 128 columns), O takes head_dim columns.  P stays there as well: narrowed to
- * BF16 it overwrites its own scores and is the MMA's A operand, so that shared memory carries Q, K and
- * V only.  (K and Q are K-major; V's rows are its K dimension: the MN-major form of the same
- * 128B-swizzled tile.)
+ * S is double-buffered in tensor memory (2 x 128 columns), O takes head_dim columns.  P stays
+ * there as well: narrowed to BF16 it overwrites its own scores and is the MMA's A operand, so that
+ * shared memory carries Q, K and V only.  (K and Q are K-major; V's rows are its K dimension: the
+ * MN-major form of the same 128B-swizzled tile.)  MMAs of one issuer run in the order of their
+ * issue: S(j+2) may overwrite the P(j) that the product before it reads.
  *
  * The maximum that a row's weights are taken against moves only when a score is 2^8 above it: any
  * reference within the range of fp32 and BF16 gives the same quotient, and O in tensor memory
@@ -37,8 +39,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "attn_decode.cuh"
 #include "attn_view.cuh"
 #include "common.cuh"
@@ -51,7 +51,8 @@ constexpr int AP_SOFT_WARPS = 8;
 constexpr int AP_THREADS = 128 + AP_SOFT_WARPS * 32;
 /* The registers of a block of twelve warps are 168 a thread.  The two warps that issue loads and
  * MMAs (and two that only fill up their group) need few; the softmax warps take over the rest:
- * 128 x 64 + 256 x 216 <= 384 x 168. */
+ * 128 x 40 + 256 x 232 = 384 x 168 (checked before the first launch: a sum above what the block has would wait
+ * for ever). */
 constexpr int AP_REGS_ISSUE = 40, AP_REGS_SOFT = 232;
 constexpr int AP_TMEM_COLS = 512;
 constexpr int AP_TMEM_O = 256;               /* scores in columns 0..255 */
@@ -91,7 +92,7 @@ struct ApItem {
     int part;                                /* with splits: whose result it is */
 };
 struct ApShared {
-    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free;
+    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free, through;
     uint64_t item_full[AP_ITEMS], item_empty[AP_ITEMS], pair[4];
     ApItem item[AP_ITEMS];
     uint32_t tmem;
@@ -218,28 +219,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-/* 2^x of two values on the FMA units, beside the 16 a cycle of the special function units:
- * x = n + f with f in [-1/2, 1/2] (n by adding 1.5 * 2^23, whose last bits are then n), 2^f by
- * its polynomial of degree 5 with the smallest largest relative error there (7.5e-8, fitted by
- * reweighted least squares), and n in the exponent of a factor.  x in [-126, 127], others as
- * the nearer end; NaN stays. */
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
-    const float2 big = make_float2(12582912.0f, 12582912.0f);
-    const float2 t = add2(x, big);
-    const float2 n = add2(t, make_float2(-12582912.0f, -12582912.0f));
-    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 y = make_float2(1.3276466634124517e-3f, 1.3276466634124517e-3f);
-    y = fma2(y, f, make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
-    y = fma2(y, f, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
-    y = fma2(y, f, make_float2(2.4022120237350464e-1f, 2.4022120237350464e-1f));
-    y = fma2(y, f, make_float2(6.931469440460205e-1f, 6.931469440460205e-1f));
-    y = fma2(y, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
-    /* (1.5 * 2^23's own bits are shifted out) */
-    return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) * 0x800000u + 0x3f800000u),
-                               __uint_as_float(__float_as_uint(t.y) * 0x800000u + 0x3f800000u)));
-}
 /* Four lanes with four pairs each: pair w of lane t to lane w, as its pair t. */
 __device__ __forceinline__ void ap_turn(uint32_t (&e)[4][2], int t) {
 #pragma unroll
@@ -347,6 +326,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             mbar_init(&s.pv_done[i], 1);
         }
         mbar_init(&s.o_free, AP_SOFT_WARPS);
+        mbar_init(&s.through, 1);
         for (int i = 0; i < AP_ITEMS; i++) {
             mbar_init(&s.item_full[i], 1);
             mbar_init(&s.item_empty[i], 1 + AP_SOFT_WARPS);
@@ -366,8 +346,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
     /* the next tile, for all roles but the one that finds it */
     auto next_item = [&](int n, ApItem &t) -> bool {
         const int i = n % AP_ITEMS;
-        if (!pg_wait(&s.item_full[i], (uint32_t)(n / AP_ITEMS) & 1u, abort_flag, p.status,
-                     ST_SCHED_TIMEOUT))
+        if (!pg_wait_warp(&s.item_full[i], (uint32_t)(n / AP_ITEMS) & 1u, abort_flag, p.status,
+                          ST_SCHED_TIMEOUT))
             return false;
         /* by shuffles, so that what follows from it (loops, descriptors) is known to be the
          * same in all lanes and is kept in uniform registers, where MMAs want it */
@@ -382,11 +362,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
     };
 
     if (warp < 4) {
+        /* (one instruction for the four warps of the group) */
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AP_REGS_ISSUE));
     if (warp == 0) {
         /* ---------------- tiles and loads ---------------- */
         uint32_t unit = 0;
-        int full = 0;                        /* tiles that see keys, so far */
+        int full = 0, asked = 0;             /* tiles that see keys, so far; of which Q was asked for */
         int index = blockIdx.x;
         bool alive = true;
         auto load = [&](bool keys, const ApItem &t, int j) {
@@ -442,6 +423,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     alive = false;
                 } else {
                     const int rows = p.a.group * p.tile_tokens;
+                    asked++;
                     mbar_expect_tx(&s.q_full, (uint32_t)(S::BLOCKS * rows * 128));
 #pragma unroll
                     for (int b = 0; b < S::BLOCKS; b++)
@@ -461,6 +443,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 index = __shfl_sync(0xffffffffu, index, 0);
             }
             alive = __all_sync(0xffffffffu, alive);
+        }
+        /* given up: copies that are under way land before the CTA leaves */
+        if (lane == 0 && *abort_flag) {
+            for (uint32_t u = unit > STAGES ? unit - STAGES : 0; u < unit; u++)
+                mbar_wait(&s.kv_full[u % STAGES], (u / STAGES) & 1u);
+            if (asked) mbar_wait(&s.q_full, (uint32_t)(asked - 1) & 1u);
         }
         /* the last CTA that asks no more sets the counters back */
         if (lane == 0 && p.items > (int)gridDim.x) {
@@ -543,8 +531,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     look_ahead();
                     const int here = min(max(keys - u * S::V_ROWS, 0), S::V_ROWS);
                     /* Keys behind the last one that any row sees have weight zero, but their
-                     * values may be anything, and 0 * NaN is not 0: whole steps of 16 of them are left out, the
-                     * rest of the last step is cleared. */
+                     * values may be anything, and 0 * NaN is not 0: whole steps of 16 of them
+                     * are left out, the rest of the last step is cleared. */
                     const int steps = (here + 15) / 16;
                     if (here & 15) {
                         unsigned char *v = ring + st * S::UNIT_BYTES;
@@ -576,6 +564,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 sums++;
             }
             full++;
+        }
+        if (*abort_flag) {                   /* given up: no MMA outlives the CTA's tensor memory */
+            if (pg_elect()) umma_commit(&s.through);
+            __syncwarp();
+            mbar_wait(&s.through, 0);
+            __syncwarp();
         }
     }
     } else {
@@ -628,8 +622,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                     tmem_ld32(ts + half * COLS + c * 32, x[c]);
                 tmem_ld_wait();
                 const int lim = sees - j * AP_ROWS - half * COLS;
-                const bool masked = !__all_sync(0xffffffffu, lim >= COLS);
-                if (masked) {
+                if (!__all_sync(0xffffffffu, lim >= COLS)) {
 #pragma unroll
                     for (int c = 0; c < COLS; c++)
                         if (c >= lim) x[c >> 5][c & 31] = 0xff800000u;
@@ -667,29 +660,20 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                 const float base = top == -INFINITY ? 0.0f : top;
                 const float2 sc2 = make_float2(sc, sc), base2 = make_float2(-base, -base);
                 float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                /* Up to head_dim 128 the exponentials are what bounds a step: every POLY-th pair
-                 * goes to the FMA units.  (Where scores are masked their weight has to be 0.) */
-                constexpr int POLY = D == 256 ? 0 : 4;
-                auto weights = [&](auto some_poly) {
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; c++) {
-                        uint32_t pk[16];
+                for (int c = 0; c < COLS / 32; c++) {
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float2 z = fma2(make_float2(__uint_as_float(x[c][2 * i]),
-                                                              __uint_as_float(x[c][2 * i + 1])),
-                                                  sc2, base2);
-                            const bool poly = some_poly.value && i % (POLY ? POLY : 1) == POLY - 1;
-                            const float2 w = poly ? exp2_poly(z)
-                                                  : make_float2(exp2_fast(z.x), exp2_fast(z.y));
-                            part[i & 1] = add2(part[i & 1], w);
-                            pk[i] = pack_bf16_rn(w.x, w.y);       /* the weights' one rounding */
-                        }
-                        tmem_st16(ts + half * (COLS / 2) + c * 16, pk);
+                    for (int i = 0; i < 16; i++) {
+                        const float2 z = fma2(make_float2(__uint_as_float(x[c][2 * i]),
+                                                          __uint_as_float(x[c][2 * i + 1])),
+                                              sc2, base2);
+                        const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                        part[i & 1] = add2(part[i & 1], w);
+                        pk[i] = pack_bf16_rn(w.x, w.y);   /* the weights' one rounding */
                     }
-                };
-                if (POLY && !masked) weights(std::true_type());
-                else weights(std::false_type());
+                    tmem_st16(ts + half * (COLS / 2) + c * 16, pk);
+                }
                 part[0] = add2(part[0], part[1]);
                 sum += part[0].x + part[0].y;
                 tmem_st_wait();

@@ -573,8 +573,9 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  * work is scratch of the calls on this cache; its first word is the cache's status, which
  * stays at the first thing that went wrong until the caller clears it: 0 ok, 1 pages ran
  * out, 2 a list names what it must not, 3 a page number outside of the pool (or a page given
- * back too often).  A kv_ call that cannot do all that its list asks for leaves everything as
- * it was (kv_free: what the bad entries name). */
+ * back too often), which is passed over where it stands in the table.  A kv_ call that cannot do
+ * all that its list asks for leaves everything as it was (kv_free: what the bad entries name).
+ * Calls on one cache are put in order by the caller: one stream, or events. */
 typedef struct {
     uint16_t *k, *v;       /* [layers][pages][kv_heads][page_tokens][head_dim] */
     int32_t *refs;         /* [pages] */
@@ -662,7 +663,10 @@ int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *key
 /* Attention of one new token a sequence over the paged cache: row b of q sees all
  * len[d_seq[b]] tokens (d_seq NULL: len[b]) of `layer`, its own among them once written.  A row
  * whose d_seq is negative stays as it is (a padded batch).  A page number outside of the pool
- * leaves its tokens out and status 3 in the cache's work. */
+ * leaves its tokens out and status 3 in the cache's work, a d_seq at or above seqs its row as it is
+ * and status 2.  One cooperative launch for 1024 rows; sums are added up in a fixed order, so equal
+ * calls give equal bits.  A wait inside that runs out: apus_cuda_last_block_status(), as for the
+ * block. */
 int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv, size_t layer,
                               const int32_t *d_seq, void *stream);
 

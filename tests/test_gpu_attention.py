@@ -319,3 +319,92 @@ def test_same_result_twice_on_streams_and_in_a_graph(gpu):
     torch.cuda.synchronize()
     for x, y in zip(first, (out, lse, pout)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_not_finite_where_a_row_looks(gpu, dim):
+    """NaN and infinity that a row does see come out as they would of the formula."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    n, H, K = 300, 8, 2
+    q, k, v = (u.normal(n, h, dim, seed=i) for i, h in enumerate((H, K, K)))
+    q[7, 3, 5] = math.nan                    # one row
+    v[20, 1, 9] = math.inf                   # a key of head 1: rows from 20 on
+    k[200, 0, 0] = math.nan                  # a key of head 0: rows from 200 on
+    out, lse = torch.empty_like(q), torch.empty(n, H, device="cuda")
+    a = u.attn(q, out, lse, kv_heads=K)
+    cu = u.ints([0, n])
+    kk = B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=n, cu_q=cu.data_ptr(),
+                    cu_k=cu.data_ptr(), seqs=1, causal=1)
+    gpu.attn_prompt_dev(a, kk, stream=u.stream())
+    torch.cuda.synchronize()
+    assert out[7, 3].isnan().all() and lse[7, 3].isnan()
+    assert out[200:, :4].isnan().all() and lse[200:, :4].isnan().all()
+    assert (out[32:, 4:, 9] == math.inf).all()
+    fine = torch.ones(n, H, dim, dtype=torch.bool, device="cuda")
+    fine[7, 3] = False
+    fine[200:, :4] = False
+    fine[:, 4:, 9] = False                   # (its tile, 128 / 4 = 32 tokens, has 0 * inf before)
+    assert out[fine].isfinite().all() and lse[:200, 4:].isfinite().all()
+    cache = u.Cache(1, 14, K, 32, dim, 2, 10).hold([n, 40])
+    for s, m in ((0, n), (1, 40)):
+        t = torch.arange(m, device="cuda")
+        at = cache.table[s, t // 32].long(), t % 32
+        cache.k[0].transpose(1, 2)[at] = k[:m]
+        cache.v[0].transpose(1, 2)[at] = v[:m]
+    q2 = u.normal(2, H, dim, seed=7)
+    out2 = torch.empty_like(q2)
+    a2 = u.attn(q2, out2, kv_heads=K)
+    gpu.attn_decode_dev(a2, cache.c, 0, None, stream=u.stream())
+    torch.cuda.synchronize()
+    assert out2[0, :4].isnan().all() and not out2[1, :4].isnan().any()
+    assert (out2[:, 4:, 9] == math.inf).all()
+
+
+def test_a_step_in_a_graph(gpu):
+    """Places, positions and cache, attention and the end of sequences captured once and replayed:
+    the same bits as the calls."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    H, K, D, page, n = 8, 2, 128, 16, 5
+    lengths = [30, 1, 15, 16, 100]
+
+    def make():
+        c = u.Cache(1, 40, K, page, D, n, 10, seed=3).hold(lengths, seed=3)
+        x = u.normal(n, H + 2 * K, D, seed=4)
+        q = torch.empty(n, H, D, dtype=torch.bfloat16, device="cuda")
+        t = dict(c=c, x=x, q=q, out=torch.empty_like(q), slot=u.ints([-1] * n),
+                 cu=u.ints(range(n + 1)), pos=u.ints([lengths]), gone=u.ints([1, 3]))
+        r = B.Rope(q=x.data_ptr(), k=x[:, H:].data_ptr(), v=x[:, H + K:].data_ptr(),
+                   q_out=q.data_ptr(), k_out=None, q_stride=x.stride(0), k_stride=x.stride(0),
+                   v_stride=x.stride(0), rows=n, heads=H, kv_heads=K, head_dim=D, rot_dim=64,
+                   pos=t["pos"].data_ptr(), axes=1, sections=(32,), theta=1e4)
+        a = u.attn(q, t["out"], kv_heads=K)
+
+        def step():
+            st = u.stream()
+            gpu.kv_extend_dev(c.c, None, t["cu"].data_ptr(), n, t["slot"].data_ptr(), n, stream=st)
+            gpu.rope_dev(r, c.c, 0, t["slot"].data_ptr(), stream=st)
+            gpu.attn_decode_dev(a, c.c, 0, None, stream=st)
+            gpu.kv_free_dev(c.c, t["gone"].data_ptr(), 2, stream=st)
+            gpu.kv_compact_dev(c.c, stream=st)
+        return t, step
+
+    one, step = make()
+    for _ in range(4):
+        step()
+    torch.cuda.synchronize()
+    two, step2 = make()
+    graph = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        step2()
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert one["c"].status() == 0 and two["c"].status() == 0
+    for x, y in zip(one["c"].state() + [one["out"], one["c"].k, one["c"].v],
+                    two["c"].state() + [two["out"], two["c"].k, two["c"].v]):
+        assert torch.equal(x, y)
