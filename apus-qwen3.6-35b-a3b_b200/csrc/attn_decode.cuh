@@ -85,10 +85,11 @@ struct AdShared {
     float m[AD_WARPS][2][AD_MAX_GROUP], l[AD_WARPS][2][AD_MAX_GROUP];
     int item[AD_WARPS][2];
     long long scan[AD_WARPS];
-    float weight[2 * AD_WARPS][AD_MAX_GROUP], top[2 * AD_WARPS][AD_MAX_GROUP],
-        sum[2 * AD_WARPS][AD_MAX_GROUP];
-    unsigned same[2 * AD_WARPS];
-    int leader[2 * AD_WARPS], leaders, joint[2];
+    /* the items that parts are of: which parts (bit 2 warp + slot), row, key head, and where the
+     * sum of them goes (0: out; else 1 + slot of shared_parts) */
+    int items, same[2 * AD_WARPS], item_row[2 * AD_WARPS], item_head[2 * AD_WARPS],
+        item_to[2 * AD_WARPS];
+    int joint[2], joint_row[2], joint_head[2], joint_first[2];    /* CTAs that hold parts of it */
 };
 inline int ad_smem_bytes() { return AD_WARPS * AD_RING_BYTES + (int)sizeof(AdShared) + 1024; }
 
@@ -162,33 +163,10 @@ __device__ __forceinline__ uint32_t ad_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void ad_store4(const AttnView &a, long row, int at, float4 y) {
-    if (a.gate) {
-        const uint2 g = *reinterpret_cast<const uint2 *>(a.gate + row * a.gate_stride + at);
-        y.x *= ad_gate(bf16lo(g.x));
-        y.y *= ad_gate(bf16hi(g.x));
-        y.z *= ad_gate(bf16lo(g.y));
-        y.w *= ad_gate(bf16hi(g.y));
-    }
-    *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + at) =
-        make_uint2(pack_bf16_rn(y.x, y.y), pack_bf16_rn(y.z, y.w));
+__device__ __forceinline__ uint2 ad_gate4(const AttnView &a, long row, int at) {
+    return a.gate ? __ldg(reinterpret_cast<const uint2 *>(a.gate + row * a.gate_stride + at))
+                  : make_uint2(0, 0);
 }
-
-/* an item, and whether a CTA's piece of the line holds all of it */
-struct AdItem {
-    int row, head;
-    long long begin, tiles;
-    bool before, after;
-    __device__ __forceinline__ AdItem(const AdShared &s, int item, int kv_heads, long long lo,
-                                      long long hi) {
-        row = item / kv_heads;
-        head = item - row * kv_heads;
-        tiles = s.start[row + 1] - s.start[row];
-        begin = s.start[row] * kv_heads + (long long)head * tiles;
-        before = begin < lo;
-        after = begin + tiles > hi;
-    }
-};
 /* (top, sum, acc) and another part's: both maxima may be of nothing */
 __device__ __forceinline__ void ad_merge(float &top, float &sum, float4 &acc, float pm, float ps,
                                          float4 v) {
@@ -203,13 +181,20 @@ __device__ __forceinline__ void ad_merge(float &top, float &sum, float4 &acc, fl
 }
 /* four values of a head's sums as they leave */
 __device__ __forceinline__ void ad_finish4(const AttnView &a, long row, int head, int D, int c,
-                                           float4 acc, float top, float sum) {
+                                           float4 y, float top, float sum, uint2 gate) {
     const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-    acc.x *= inv;
-    acc.y *= inv;
-    acc.z *= inv;
-    acc.w *= inv;
-    ad_store4(a, row, head * D + c, acc);
+    y.x *= inv;
+    y.y *= inv;
+    y.z *= inv;
+    y.w *= inv;
+    if (a.gate) {
+        y.x *= ad_gate(bf16lo(gate.x));
+        y.y *= ad_gate(bf16hi(gate.x));
+        y.z *= ad_gate(bf16lo(gate.y));
+        y.w *= ad_gate(bf16hi(gate.y));
+    }
+    *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + head * D + c) =
+        make_uint2(pack_bf16_rn(y.x, y.y), pack_bf16_rn(y.z, y.w));
     if (c == 0 && a.lse)
         a.lse[row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
@@ -226,16 +211,17 @@ __device__ __forceinline__ uint4 ad_look2(const uint2 *at) {
                  : "memory");
     return v;
 }
-/* four values and a head's max and sum of this round, for about a second at most */
+/* Four values and a head's max and sum, looked at once already: again until they are this
+ * round's, for about a second at most. */
 __device__ __forceinline__ bool ad_get(const uint2 *at, const uint2 *at_ml, unsigned round,
                                        uint4 &a, uint4 &b, uint4 &ml) {
     for (uint32_t i = 0; i < APUS_WAIT_LIMIT; i++) {
-        a = ad_look2(at);
-        b = ad_look2(at + 2);
-        ml = ad_look2(at_ml);
         if (a.y == round && a.w == round && b.y == round && b.w == round && ml.y == round &&
             ml.w == round)
             return true;
+        a = ad_look2(at);
+        b = ad_look2(at + 2);
+        ml = ad_look2(at_ml);
         if (i > 64) __nanosleep(64);
     }
     return false;
@@ -402,23 +388,27 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 for (int j = 0; j < 4; j++) o[n][k][j] = 0.0f;
         }
     };
-    /* an unfinished result in fp32 */
-    auto leave = [&](float *dst, int slot) {
+    auto leave_top = [&](int slot) {
+        if (t4 == 0)
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+            for (int n = 0; n < NT; n++) {
+                s.m[warp][slot][n * 8 + g] = m[n];
+                s.l[warp][slot][n * 8 + g] = l[n];
+            }
+    };
+    /* an unfinished result in fp32, times a factor for each head */
+    auto leave = [&](float *dst, const float (&f)[NT][2]) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int h = n * 8 + t4 * 2 + (j & 1);
                 if (h < group)
 #pragma unroll
                     for (int k = 0; k < MT; k++)
-                        dst[h * (D + AD_PAD) + k * 16 + (j >> 1) * 8 + g] = o[n][k][j];
+                        dst[h * (D + AD_PAD) + k * 16 + (j >> 1) * 8 + g] =
+                            o[n][k][j] * f[n][j & 1];
             }
-            if (t4 == 0) {
-                s.m[warp][slot][n * 8 + g] = m[n];
-                s.l[warp][slot][n * 8 + g] = l[n];
-            }
-        }
     };
     const size_t warp_part = (size_t)(blockIdx.x * AD_WARPS + warp) * AD_PART_FLOATS;
     bool first = cc.tile > 0;              /* the item began before this piece */
@@ -577,10 +567,15 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                                       k * 8) = y;
                 }
             }
-        } else if (done == to) {                          /* in the ring, once all is through */
+        } else if (done == to) {                          /* kept until all is through */
+            leave_top(1);
             if (lane == 0) s.item[warp][1] = item;
         } else {                                          /* out of the way of what comes */
-            leave(p.parts + warp_part, 0);
+            float one[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) one[n][0] = one[n][1] = 1.0f;
+            leave(p.parts + warp_part, one);
+            leave_top(0);
             if (lane == 0) s.item[warp][0] = item;
         }
         first = false;
@@ -595,100 +590,114 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             mbar_wait(&s.full[warp][used % STAGES], (used / STAGES) & 1u);
     }
     __syncthreads();                                      /* every ring is read to its end */
-    float *mine = reinterpret_cast<float *>(ring0) + warp * (AD_RING_BYTES / 4);
-    if (s.item[warp][1] >= 0) leave(mine, 1);
-    __syncthreads();
 
-    /* ---- the SM's unfinished results, put together in the order of the line ---- */
-    /* (Loops over the set bits of an entry's mask, not unrolled: what runs once or twice is bound
-     * by its instructions' way out of L2.) */
+    /* ---- the SM's unfinished results, put together in the order of the line ----
+     * What this takes is mostly instructions that run once, out of L2 at 8 cycles each: few of
+     * them, and nothing that an earlier step can say. */
     constexpr int ENTRIES = 2 * AD_WARPS;
-    static_assert(ENTRIES == 16, "entries are lanes and bits");
-    if (tid < ENTRIES) {
+    if (tid < 2) s.joint[tid] = 0;
+    __syncwarp();
+    if (tid < ENTRIES) {                                  /* an entry to a lane */
         const int item = s.item[tid >> 1][tid & 1];
-        const unsigned same = __match_any_sync(0xffffu, item);        /* entries of the same item */
+        const unsigned same = __match_any_sync(0xffffu, item);
         const bool leads = item >= 0 && __ffs(same) - 1 == tid;
         const unsigned leaders = __ballot_sync(0xffffu, leads);
-        s.same[tid] = same;
-        if (leads) s.leader[__popc(leaders & ((1u << tid) - 1))] = tid;
-        if (tid == 0) s.leaders = __popc(leaders);
-    }
-    __syncthreads();
-    const int items = s.leaders;
-    {                                                     /* the weight of an entry's head */
-        const int e = tid / AD_MAX_GROUP, h = tid % AD_MAX_GROUP;
-        if (s.item[e >> 1][e & 1] >= 0 && h < group) {
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll 1
-            for (unsigned b = s.same[e]; b; b &= b - 1) {
-                const int j = __ffs(b) - 1;
-                top = fmaxf(top, s.m[j >> 1][j & 1][h]);
+        if (tid == 0) s.items = __popc(leaders);
+        if (leads) {
+            const int i = __popc(leaders & ((1u << tid) - 1));
+            const int row = item / p.kv_heads, head = item - row * p.kv_heads;
+            const long long tiles = s.start[row + 1] - s.start[row],
+                            begin = s.start[row] * p.kv_heads + head * tiles;
+            const bool before = begin < lo, after = begin + tiles > hi;
+            s.same[i] = same;
+            s.item_row[i] = row;
+            s.item_head[i] = head;
+            s.item_to[i] = before ? 1 : after ? 2 : 0;
+            if (before || after) {
+                const int j = !before, c0 = ad_piece_of(begin, per);
+                s.joint_first[j] = c0;
+                s.joint[j] = ad_piece_of(begin + tiles - 1, per) - c0 + 1;
+                s.joint_row[j] = row;
+                s.joint_head[j] = head;
             }
-            if (top == -INFINITY) top = 0.0f;             /* nothing counted: weights of 0 */
-#pragma unroll 1
-            for (unsigned b = s.same[e]; b; b &= b - 1) {
-                const int j = __ffs(b) - 1;
-                sum = fmaf(exp2_fast(s.m[j >> 1][j & 1][h] - top), s.l[j >> 1][j & 1][h], sum);
-            }
-            s.weight[e][h] = exp2_fast(s.m[e >> 1][e & 1][h] - top);
-            s.top[e][h] = top;
-            s.sum[e][h] = sum;
         }
+    }
+    const int mine = s.item[warp][1];
+    if (mine >= 0) {                                      /* in the ring, against the item's maximum */
+        float f[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int h = n * 8 + t4 * 2 + j;
+                float top = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < ENTRIES; e++)
+                    if (s.item[e >> 1][e & 1] == mine) top = fmaxf(top, s.m[e >> 1][e & 1][h]);
+                f[n][j] = exp2_fast(s.m[warp][1][h] - (top == -INFINITY ? 0.0f : top));
+            }
+        leave(reinterpret_cast<float *>(ring0 + warp * AD_RING_BYTES), f);
     }
     __syncthreads();
     constexpr int HEAD4 = D / 4;                          /* pieces of 16 bytes of a head */
-    const int per_item = group * HEAD4;
+    const int per_item = group * HEAD4, pieces_here = s.items * per_item;
 #pragma unroll 1
-    for (int x = tid; x < items * per_item; x += AD_THREADS) {
-        const int nth = x / per_item, in = x - nth * per_item;
-        const int h = in / HEAD4, c = (in - h * HEAD4) * 4;
-        const int e = s.leader[nth], item = s.item[e >> 1][e & 1];
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-        for (unsigned b = s.same[e]; b; b &= b - 1) {
-            const int j = __ffs(b) - 1, w = j >> 1;
-            const float f = s.weight[j][h];
-            const int from_at = h * (D + AD_PAD) + c;
-            const float4 v = j & 1
-                                 ? *reinterpret_cast<const float4 *>(ring0 + w * AD_RING_BYTES +
-                                                                     from_at * 4)
-                                 : *reinterpret_cast<const float4 *>(
-                                       p.parts + (size_t)(blockIdx.x * AD_WARPS + w) *
-                                                     AD_PART_FLOATS + from_at);
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
+    for (int x = tid; x < pieces_here; x += AD_THREADS) {
+        int i = 0, in = x;
+        for (; in >= per_item; in -= per_item) i++;
+        const int h = in / HEAD4, c = (in - h * HEAD4) * 4, at = h * (D + AD_PAD) + c;
+        const unsigned same = s.same[i];
+        float4 v[AD_WARPS], acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AD_WARPS; w++) {
+            const bool of = same >> (2 * w + 1) & 1;
+            v[w] = of ? *reinterpret_cast<const float4 *>(ring0 + w * AD_RING_BYTES + at * 4)
+                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (of) top = fmaxf(top, s.m[w][1][h]);
         }
-        const AdItem it(s, item, p.kv_heads, lo, hi);
-        const float top = s.top[e][h], sum = s.sum[e][h];
-        if (it.before || it.after) {
-            uint2 *part = p.shared_parts + (size_t)(blockIdx.x * 2 + !it.before) * AD_SHARED_WORDS;
+        for (unsigned b = same & 0x5555u; b; b &= b - 1)
+            top = fmaxf(top, s.m[(__ffs(b) - 1) >> 1][0][h]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < AD_WARPS; w++) {
+            if (same >> (2 * w + 1) & 1) sum = fmaf(exp2_fast(s.m[w][1][h] - base), s.l[w][1][h], sum);
+            acc.x += v[w].x;
+            acc.y += v[w].y;
+            acc.z += v[w].z;
+            acc.w += v[w].w;
+        }
+        for (unsigned b = same & 0x5555u; b; b &= b - 1) {        /* what ended in a warp */
+            const int w = (__ffs(b) - 1) >> 1;
+            const float f = exp2_fast(s.m[w][0][h] - base);
+            const float4 y = *reinterpret_cast<const float4 *>(
+                p.parts + (size_t)(blockIdx.x * AD_WARPS + w) * AD_PART_FLOATS + at);
+            sum = fmaf(f, s.l[w][0][h], sum);
+            acc.x = fmaf(f, y.x, acc.x);
+            acc.y = fmaf(f, y.y, acc.y);
+            acc.z = fmaf(f, y.z, acc.z);
+            acc.w = fmaf(f, y.w, acc.w);
+        }
+        const int dest = s.item_to[i];
+        if (dest) {
+            uint2 *part = p.shared_parts + (size_t)(blockIdx.x * 2 + dest - 1) * AD_SHARED_WORDS;
             ad_put2(part + h * D + c, acc.x, acc.y, round);
             ad_put2(part + h * D + c + 2, acc.z, acc.w, round);
             if (c == 0) ad_put2(part + AD_SHARED_ML + 2 * h, top, sum, round);
         } else {
-            ad_finish4(p.a, p.row0 + it.row, it.head * group + h, D, c, acc, top, sum);
+            const long row = p.row0 + s.item_row[i];
+            const int head = s.item_head[i] * group + h;
+            ad_finish4(p.a, row, head, D, c, acc, top, sum, ad_gate4(p.a, row, head * D + c));
         }
     }
 
     /* ---- items that several SMs hold parts of ---- */
-    if (tid < 2) s.joint[tid] = -1;
-    __syncthreads();
-    if (tid < items) {
-        const int e = s.leader[tid], item = s.item[e >> 1][e & 1];
-        const AdItem it(s, item, p.kv_heads, lo, hi);
-        if (it.before || it.after) s.joint[!it.before] = item;
-    }
-    __syncthreads();
     bool gone = false;                                    /* a part that never came: ask for no other */
 #pragma unroll 1
     for (int j = 0; j < 2; j++) {
-        const int item = s.joint[j];
-        if (item < 0) continue;
-        const AdItem it(s, item, p.kv_heads, lo, hi);
-        const int c0 = ad_piece_of(it.begin, per),
-                  n = ad_piece_of(it.begin + it.tiles - 1, per) - c0 + 1;
+        const int n = s.joint[j], c0 = s.joint_first[j];
+        if (!n) continue;
+        const long row = p.row0 + s.joint_row[j];
         /* every SM that holds a part adds up a share of the pieces: a few lanes to a piece, each
          * some of the parts, then the lanes by shuffles */
         const int share = (per_item + n - 1) / n, first_piece = share * ((int)blockIdx.x - c0);
@@ -701,21 +710,38 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
         for (int x0 = tid / lanes; x0 - tid / lanes < pieces; x0 += AD_THREADS / lanes) {
             const bool real = x0 < pieces;
             const int in = first_piece + (real ? x0 : 0), h = in / HEAD4, c = (in - h * HEAD4) * 4;
+            const int head = s.joint_head[j] * group + h;
+            const uint2 gate = ad_gate4(p.a, row, head * D + c);      /* beside the wait */
             float top = -INFINITY, sum = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-            for (int e = sub; e < n && !gone; e += lanes) {
-                const uint2 *part =
-                    p.shared_parts + (size_t)((c0 + e) * 2 + (e == 0)) * AD_SHARED_WORDS;
-                uint4 a, b, ml;
-                if (!ad_get(part + h * D + c, part + AD_SHARED_ML + 2 * h, round, a, b, ml)) {
-                    set_status(p.wait_status, ST_SCHED_TIMEOUT);
-                    gone = true;
-                    break;
+            for (int e0 = sub; e0 < n && !gone; e0 += 2 * lanes) {
+                uint4 a[2], b[2], ml[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {             /* both under way before one is waited for */
+                    const int e = min(e0 + k * lanes, n - 1);
+                    const uint2 *part =
+                        p.shared_parts + (size_t)((c0 + e) * 2 + (e == 0)) * AD_SHARED_WORDS;
+                    a[k] = ad_look2(part + h * D + c);
+                    b[k] = ad_look2(part + h * D + c + 2);
+                    ml[k] = ad_look2(part + AD_SHARED_ML + 2 * h);
                 }
-                ad_merge(top, sum, acc, __uint_as_float(ml.x), __uint_as_float(ml.z),
-                         make_float4(__uint_as_float(a.x), __uint_as_float(a.z),
-                                     __uint_as_float(b.x), __uint_as_float(b.z)));
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int e = e0 + k * lanes;
+                    if (e >= n || gone) continue;
+                    const uint2 *part =
+                        p.shared_parts + (size_t)((c0 + e) * 2 + (e == 0)) * AD_SHARED_WORDS;
+                    if (!ad_get(part + h * D + c, part + AD_SHARED_ML + 2 * h, round, a[k], b[k],
+                                ml[k])) {
+                        set_status(p.wait_status, ST_SCHED_TIMEOUT);
+                        gone = true;
+                        continue;
+                    }
+                    ad_merge(top, sum, acc, __uint_as_float(ml[k].x), __uint_as_float(ml[k].z),
+                             make_float4(__uint_as_float(a[k].x), __uint_as_float(a[k].z),
+                                         __uint_as_float(b[k].x), __uint_as_float(b[k].z)));
+                }
             }
             for (int o = 1; o < lanes; o <<= 1) {
                 float4 v;
@@ -727,8 +753,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                 v.w = __shfl_xor_sync(0xffffffffu, acc.w, o);
                 ad_merge(top, sum, acc, pm, ps, v);
             }
-            if (real && sub == 0)
-                ad_finish4(p.a, p.row0 + it.row, it.head * group + h, D, c, acc, top, sum);
+            if (real && sub == 0) ad_finish4(p.a, row, head, D, c, acc, top, sum, gate);
         }
     }
     if (tid == 0 && seen == gridDim.x - 1) atomicAdd(p.sync + AD_SYNC_ROUND, 1u);
