@@ -11,7 +11,7 @@
  * vectors, finds the cosines and sines, a pair to a lane, while they are under way (in turns,
  * reduced in 64 bits: at position 10^6 a 32-bit angle is off by 0.06), and keeps those of its lanes' values in
  * registers.  A lane holds 16 bytes of a head; the other half of its pairs is in a lane r/16
- * away.  8192 tokens of 16 + 2 + 2 heads of 256: 28 us, 145 MB at 5.2 TB/s.
+ * away.  6732 tokens of 16 + 2 + 2 heads of 256: 28 us, 145 MB at 5.2 TB/s.
  */
 #pragma once
 #include <cuda_runtime.h>
