@@ -405,9 +405,9 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     if (ord.rc) return 1;
     /* Tiles that leave SMs idle share their keys, by four steps of 128 at least: the second kernel
      * takes as long as two or three.  head_dim 256, 2 key heads: 16 rows over 4096 keys 52 -> 31
-     * us, 128 rows over 30128 331 -> 77, one row over 1000 20 -> 17.  Where the parts would fill the SMs, their way
-     * through memory takes longer than a few steps: 400 rows over 1000 keys 21 -> 26, so only
-     * from sixteen steps on. */
+     * us, 128 rows over 30128 331 -> 77, one row over 1000 20 -> 17.  Where the parts would fill
+     * the SMs, their way through memory takes longer than a few steps: 400 rows over 1000 keys 21
+     * -> 26, so only from sixteen steps on. */
     size_t splits = (size_t)c->sm_count / p.items;
     if (splits > steps / 4) splits = steps / 4;
     if (splits > AP_MAX_SPLITS) splits = AP_MAX_SPLITS;

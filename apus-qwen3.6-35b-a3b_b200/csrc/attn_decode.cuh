@@ -692,7 +692,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     }
 
     /* ---- items that several SMs hold parts of ---- */
-    bool gone = false;                                    /* a part that never came: ask for no other */
+    bool gone = false;                                    /* a part never came: ask for no other */
 #pragma unroll 1
     for (int j = 0; j < 2; j++) {
         const int n = s.joint[j], c0 = s.joint_first[j];

@@ -51,8 +51,8 @@ constexpr int AP_SOFT_WARPS = 8;
 constexpr int AP_THREADS = 128 + AP_SOFT_WARPS * 32;
 /* The registers of a block of twelve warps are 168 a thread.  The two warps that issue loads and
  * MMAs (and two that only fill up their group) need few; the softmax warps take over the rest:
- * 128 x 40 + 256 x 232 = 384 x 168 (checked before the first launch: a sum above what the block has would wait
- * for ever). */
+ * 128 x 40 + 256 x 232 = 384 x 168 (checked before the first launch: a sum above what the block
+ * has would wait for ever). */
 constexpr int AP_REGS_ISSUE = 40, AP_REGS_SOFT = 232;
 constexpr int AP_TMEM_COLS = 512;
 constexpr int AP_TMEM_O = 256;               /* scores in columns 0..255 */
@@ -77,9 +77,9 @@ struct PromptParams {
     const int32_t *cu_q, *cu_k;
     int k_rows, seqs, causal, kv_heads;
     int tile_tokens;                         /* 128 / group */
-    int slots, items;                        /* tiles that there may be, times key heads and splits */
+    int slots, items;                        /* tiles there may be, times key heads and splits */
     int splits;                              /* CTAs that share a tile's keys */
-    float *parts;                            /* with splits: their results, [items][AP_PART_FLOATS] */
+    float *parts;                            /* with splits: [items][AP_PART_FLOATS] */
     unsigned *sched;                         /* next item; [32]: CTAs that are through */
     int *status;
 };
@@ -92,7 +92,8 @@ struct ApItem {
     int part;                                /* with splits: whose result it is */
 };
 struct ApShared {
-    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free, through;
+    uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free,
+        through;
     uint64_t item_full[AP_ITEMS], item_empty[AP_ITEMS], pair[4];
     ApItem item[AP_ITEMS];
     uint32_t tmem;
@@ -367,7 +368,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
     if (warp == 0) {
         /* ---------------- tiles and loads ---------------- */
         uint32_t unit = 0;
-        int full = 0, asked = 0;             /* tiles that see keys, so far; of which Q was asked for */
+        int full = 0, asked = 0;             /* tiles that see keys; those whose Q was asked for */
         int index = blockIdx.x;
         bool alive = true;
         auto load = [&](bool keys, const ApItem &t, int j) {

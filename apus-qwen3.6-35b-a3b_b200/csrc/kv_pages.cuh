@@ -14,7 +14,8 @@
  * depend on one another (about 0.7 us each), so refs is asked for before the list, and marks of
  * sequences are bits in shared memory.  A plan that cannot be carried out leaves a status and
  * changes nothing.  What moves bytes (kv_apply_kernel) runs on all SMs and reads the plan: its
- * bound is HBM, each page read once and written once (482 MB of pages moved together: 75 us, 6.4 TB/s).
+ * bound is HBM, each page read once and written once (241 MB moved together: 75 us, 6.4 TB/s of
+ * reads and writes).
  */
 #pragma once
 #include <cuda_runtime.h>

@@ -7,11 +7,11 @@
  *   what lies behind the first r values of a head is passed on.
  *
  * Bound: HBM (each vector read once, written once or twice).  The angles are the same for all
- * heads of a token, so a warp takes a token (or, with few tokens, several warps one): it asks for its first
- * vectors, finds the cosines and sines, a pair to a lane, while they are under way (in turns,
- * reduced in 64 bits: at position 10^6 a 32-bit angle is off by 0.06), and keeps those of its lanes' values in
- * registers.  A lane holds 16 bytes of a head; the other half of its pairs is in a lane r/16
- * away.  6732 tokens of 16 + 2 + 2 heads of 256: 28 us, 145 MB at 5.2 TB/s.
+ * heads of a token, so a warp takes a token (or, with few tokens, several warps one): it asks for
+ * its first vectors, finds the cosines and sines, a pair to a lane, while they are under way (in
+ * turns, reduced in 64 bits: at position 10^6 a 32-bit angle is off by 0.06), and keeps those of
+ * its lanes' values in registers.  A lane holds 16 bytes of a head; the other half of its pairs is
+ * in a lane r/16 away.  6728 tokens of 16 + 2 + 2 heads of 256: 28 us, 145 MB at 5.2 TB/s.
  */
 #pragma once
 #include <cuda_runtime.h>

@@ -566,8 +566,8 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  *     ((l * pages + p) * kv_heads + h) * page_tokens * head_dim
  * of k and of v.  Token t of sequence s is token t % page_tokens of page
  * table[s * max_pages + t / page_tokens].  refs counts the sequences that hold a page, 0 is a
- * free one.  A new cache has refs 0, len 0, table -1 and work 0 (k and v as they are).  Entries of the table behind a
- * sequence's last page are not read.  pages * kv_heads * page_tokens < 2^31,
+ * free one.  A new cache has refs 0, len 0, table -1 and work 0 (k and v as they are).  Entries of
+ * the table behind a sequence's last page are not read.  pages * kv_heads * page_tokens < 2^31,
  * seqs at most 65536.
  *
  * work is scratch of the calls on this cache; its first word is the cache's status, which
@@ -599,8 +599,8 @@ int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, con
  * two owners is ever written. */
 int apus_cuda_kv_fork_dev(const ApusCudaKvCache *kv, const int32_t *d_src, const int32_t *d_dst,
                           size_t n, void *stream);
-/* Sequences d_seq[i] (NULL: i) end: their length is 0, their pages have one owner less, their entries of
- * the table are -1. */
+/* Sequences d_seq[i] (NULL: i) end: their length is 0, their pages have one owner less, their
+ * entries of the table are -1. */
 int apus_cuda_kv_free_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, size_t n,
                           void *stream);
 /* The pages in use move to the front of the pool: those at or behind the number of pages in
