@@ -98,8 +98,7 @@ struct ApShared {
     ApItem item[AP_ITEMS];
     uint32_t tmem;
     int abort_flag;
-    uint16_t top[2][2][AP_ROWS];             /* a step's maxima, BF16: a reference needs no more */
-    float sum[2][AP_ROWS];
+    float shown[2][2][AP_ROWS];              /* what a pair of warps tells one another, in turns */
 };
 template <int D>
 constexpr int ap_smem_bytes() {
@@ -592,11 +591,17 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             tc_fence_after();
             return alive;
         };
-        auto exchange = [&]() {
+        /* a row's other half; two buffers in turns: who writes one has seen the other warp through
+         * with it, at the exchange between */
+        auto exchange = [&](float &x) {
+            float (&shown)[2][AP_ROWS] = s.shown[rounds & 1u];
+            shown[half][row] = x;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.pair[quarter]);
-            return wait(&s.pair[quarter], rounds++);
+            if (!wait(&s.pair[quarter], rounds++)) return false;
+            x = shown[half ^ 1][row];
+            return true;
         };
         /* O holds step i.  A parity tells a phase only from the one before it, and that this warp
          * (or its pair) has seen i's scores says no more than that step i - 2 is through: two
@@ -632,11 +637,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
                 for (int c = 0; c < COLS; c++)
                     mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c >> 5][c & 31]));
-                const uint16_t m16 = (uint16_t)pack_bf16_rn(
-                    fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc, 0.0f);
-                s.top[buf][half][row] = m16;
-                if (!exchange()) break;
-                const float m = fmaxf(bf16_f32(m16), bf16_f32(s.top[buf][half ^ 1][row]));
+                const float m_here = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                float m = m_here;
+                if (!exchange(m)) break;
+                m = fmaxf(m, m_here);
                 const bool move = m > top + 8.0f || (top == -INFINITY && m > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
                     const float f = move ? exp2_fast(top - m) : 1.0f;
@@ -715,9 +719,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
             };
             if (p.a.gate && !SPLIT) load_gate(0);
             if (t.tiles) {
-                s.sum[half][row] = sum;
-                if (!exchange()) break;
-                sum += s.sum[half ^ 1][row];
+                float other = sum;
+                if (!exchange(other)) break;
+                sum += other;
                 if (!wait_outputs(first + t.tiles - 1)) break;
             }
             const float inv = __fdividef(1.0f, sum);

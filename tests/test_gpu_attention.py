@@ -119,6 +119,49 @@ def test_prompt_rising_keys(gpu, dim):
     u.check(out, lse, ref)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,keys", [(300, 300), (5, 3000), (1, 700)])
+@pytest.mark.parametrize("unit", [32.0, 2.0 ** 16])
+def test_scores_far_from_zero(gpu, dim, rows, keys, unit):
+    """Scores up to 8128 units (2^29), 64 of them apart at least, both signs: a softmax takes the largest
+    one, wherever it is, and splits evenly among equal ones.  The products are exact in fp32, so
+    that what is left are a weight's rounding and the result's, 2^-8 each, and for lse those of
+    (score log2(e) + log2(sum)) ln(2), a step of fp32 each."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    H, g = 4, torch.Generator().manual_seed(rows)
+    q = torch.zeros(rows, H, dim, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 64.0
+    k = torch.zeros(keys, 1, dim, dtype=torch.bfloat16, device="cuda")
+    k[:, 0, 0] = (torch.randint(-127, 128, (keys,), generator=g) * unit).bfloat16().cuda()
+    v = u.normal(keys, 1, dim, seed=1)
+    out, lse = torch.empty_like(q), torch.empty(rows, H, device="cuda")
+    cq, ck = u.ints([0, rows]), u.ints([0, keys])
+    gpu.attn_prompt_dev(u.attn(q, out, lse, kv_heads=1, scale=1.0),
+                        B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=keys, cu_q=cq.data_ptr(),
+                                   cu_k=ck.data_ptr(), seqs=1, causal=1), stream=u.stream())
+    cache = u.Cache(1, 200, 1, 16, dim, 1, 200).hold([keys])
+    pages = cache.table[0, :-(-keys // 16)].long()
+    fill = torch.zeros(2, len(pages) * 16, dim, dtype=torch.bfloat16, device="cuda")
+    fill[0, :keys], fill[1, :keys] = k[:, 0], v[:, 0]
+    cache.k[0, pages, 0], cache.v[0, pages, 0] = fill.view(2, -1, 16, dim).unbind(0)
+    one, one_lse = torch.empty_like(q[:1]), torch.empty(1, H, device="cuda")
+    gpu.attn_decode_dev(u.attn(q[-1:], one, one_lse, kv_heads=1, scale=1.0), cache.c, 0,
+                        stream=u.stream())
+    torch.cuda.synchronize()
+    assert gpu.last_block_status() == 0 and cache.status() == 0
+    score = 64.0 * k[:, 0, 0].double()
+    for i in range(rows):
+        seen = score[:keys - rows + 1 + i]
+        at = (seen == seen.max()).nonzero()[:, 0]
+        want, size = v[at, 0].double().mean(0), v[at, 0].double().abs().mean(0)
+        want_lse = float(seen.max()) + math.log(len(at))
+        for o, l in [(out[i], lse[i])] + ([(one[0], one_lse[0])] if i == rows - 1 else []):
+            assert ((o.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * size).all()
+            assert ((l.double() - want_lse).abs() <= 2.0 ** -21 * abs(want_lse) + 2.0 ** -20).all()
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 8, 128), (8, 1, 64)])
 def test_prompt_not_finite_where_nothing_sees(gpu, heads, kv_heads, dim):
     """NaN and infinity behind the last key, and in the sequences beside a sound one."""
