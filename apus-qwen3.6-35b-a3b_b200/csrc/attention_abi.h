@@ -33,7 +33,8 @@ static int kv_view(const ApusCudaKvCache *kv, const char *what, KvView *out) {
         return fail("%s: the pools must be 16-byte aligned", what);
     const size_t most = 0x7fffffff;
     if (kv->kv_heads > 1024 || kv->pages > most / (kv->page_tokens * kv->kv_heads) ||
-        kv->max_pages > most / kv->page_tokens || kv->layers > 65536 || kv->seqs > (size_t)KV_MAX_SEQS ||
+        kv->max_pages > most / kv->page_tokens || kv->layers > 65536 ||
+        kv->seqs > (size_t)KV_MAX_SEQS || kv->max_pages > most / kv->seqs ||
         kv->kv_heads * kv->page_tokens > most / kv->head_dim)
         return fail("%s: the cache is too large", what);
     KvView v;
@@ -193,8 +194,8 @@ extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *
     if (heads_check("rope_dev", r->heads, r->kv_heads, r->head_dim)) return 1;
     if (!r->rot_dim || r->rot_dim % 16 || r->rot_dim > r->head_dim)
         return fail("rope_dev: rot_dim must be a multiple of 16, at most head_dim");
-    if (!r->axes || r->axes > 4 || !(r->theta > 0.0) || r->theta > 1e30)
-        return fail("rope_dev: 1 to 4 axes and a positive theta");
+    if (!r->axes || r->axes > 4 || !(r->theta >= 1.0) || r->theta > 1e30)
+        return fail("rope_dev: 1 to 4 axes and a theta of 1 to 1e30");
     RopeParams p = {};
     const size_t pairs = r->rot_dim / 2;
     size_t count[4] = {}, sum = 0;
@@ -242,6 +243,9 @@ extern "C" int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *
         (!kv && !r->k_out))
         return fail("rope_dev: a tensor is missing, or its address or stride is not a multiple "
                     "of 16 bytes or less than a row");
+    if ((r->q == r->q_out && p.q_stride != p.q_out_stride) ||
+        (r->k == r->k_out && p.k_stride != p.k_out_stride))
+        return fail("rope_dev: in place needs equal strides");
     p.q = r->q;
     p.k = r->k;
     p.v = r->v;

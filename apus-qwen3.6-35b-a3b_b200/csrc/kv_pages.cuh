@@ -284,7 +284,9 @@ kv_fork_plan_kernel(KvView kv, const int32_t *__restrict__ src, const int32_t *_
                     bad = 1;
                 } else {
                     const int tokens = kv.len[s];
-                    if (tokens < 0 || kv.len[dst[i]] != 0) bad = 1;
+                    if (tokens < 0 || tokens > kv.max_pages * kv.page_tokens ||
+                        kv.len[dst[i]] != 0)
+                        bad = 1;
                     else need = tokens % kv.page_tokens ? 1 : 0;
                 }
             }

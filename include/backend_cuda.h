@@ -554,7 +554,8 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  * Net-new beside the engine's CPU kernels (c/attn.h: one sequence, one plain cache): what a
  * server needs between the projections of a full-attention layer.  All pointers are device
  * pointers of the backend's device, BF16 tensors as codes; calls enqueue on `stream`, do not
- * synchronise, allocate nothing once the backend is enabled, and may be captured in a graph.
+ * synchronise, allocate nothing once the backend is enabled, and may be captured in a graph
+ * (attention sums up in the shared workspace: one stream order of graphs, as for the block).
  * Tensors are addressed by rows: `stride` elements from one row (token) to the next (0: heads *
  * head_dim), heads side by side within a row; addresses and strides in multiples of 16 bytes.
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 times as many: head h
@@ -567,8 +568,8 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  * of k and of v.  Token t of sequence s is token t % page_tokens of page
  * table[s * max_pages + t / page_tokens].  refs counts the sequences that hold a page, 0 is a
  * free one.  A new cache has refs 0, len 0, table -1 and work 0 (k and v as they are).  Entries of
- * the table behind a sequence's last page are not read.  pages * kv_heads * page_tokens < 2^31,
- * seqs at most 65536.
+ * the table behind a sequence's last page are not read.  pages * kv_heads * page_tokens
+ * and seqs * max_pages < 2^31, seqs at most 65536.
  *
  * work is scratch of the calls on this cache; its first word is the cache's status, which
  * stays at the first thing that went wrong until the caller clears it: 0 ok, 1 pages ran
@@ -624,7 +625,7 @@ typedef struct {
     const int32_t *pos;               /* [axes][rows] */
     size_t axes, sections[4];
     int interleaved;
-    double theta;
+    double theta;                     /* 1 to 1e30 */
 } ApusCudaRope;
 /* With kv: the rotated keys and the values also go to place d_slot[row] of `layer` (negative:
  * nowhere; see apus_cuda_kv_extend_dev; no place twice).  kv NULL: no cache, d_slot is not read. */
@@ -633,8 +634,8 @@ int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *kv, size_t 
 
 /* What both forms of attention take: s_j = scale q . k_j over the keys that a row sees,
  * p = softmax(s), out = (sum_j p_j v_j) * sigmoid(gate), narrowed once; lse = log sum_j exp(s_j).
- * Sums and statistics are fp32; p is narrowed to BF16 for its product with v.  A row that sees no
- * key gets zeros and -inf.  out overlaps no input. */
+ * Sums and statistics are fp32 (|s_j| below 2^30); p is narrowed to BF16 for its product
+ * with v.  A row that sees no key gets zeros and -inf.  out overlaps no input. */
 typedef struct {
     const uint16_t *q;                /* [rows][heads][head_dim] */
     const uint16_t *gate;             /* the same, or NULL: no gate */

@@ -107,6 +107,19 @@ def test_rope_is_refused(be, B, bad):
         be.rope_dev(rope(B, **bad))
 
 
+@pytest.mark.parametrize("bad", [
+    dict(theta=0.5), dict(theta=1e31), dict(q=BIG, q_out=BIG, q_out_stride=512),
+    dict(k=BIG, k_out=BIG, k_stride=512)])
+def test_rope_is_refused_outside_of_its_ranges(be, B, bad):
+    with pytest.raises(B.BackendError, match="theta|equal strides"):
+        be.rope_dev(rope(B, **bad))
+
+
+def test_a_table_too_large_to_count_is_refused(be, B):
+    with pytest.raises(B.BackendError, match="too large"):
+        be.kv_free_dev(cache(B, seqs=1 << 10, max_pages=1 << 21), BIG, 1)
+
+
 def test_rope_and_cache_have_to_agree(be, B):
     for r, c, layer, slot in ((rope(B), cache(B, kv_heads=1), 0, BIG),
                               (rope(B), cache(B), 1, BIG), (rope(B), cache(B), 0, None),

@@ -206,6 +206,17 @@ def test_lists_that_are_refused_change_nothing(gpu):
     assert int(cache.refs.sum()) == 4
 
 
+def test_a_length_beyond_the_table_is_not_forked(gpu):
+    import torch
+    import attn_util as u
+    cache = u.Cache(1, 8, 1, 16, 64, 3, 2)
+    cache.len[1] = 33                                     # two pages hold 32
+    before, (src, dst) = cache.state(), (u.ints([1]), u.ints([0]))
+    gpu.kv_fork_dev(cache.c, src.data_ptr(), dst.data_ptr(), 1, stream=u.stream())
+    assert cache.status() == 2
+    assert all(torch.equal(x, y) for x, y in zip(before, cache.state()))
+
+
 @pytest.mark.parametrize("pages,n,layers,kv_heads,page,dim", [
     (400, 190, 3, 2, 32, 128), (12000, 4500, 1, 1, 16, 64), (300000, 40, 1, 1, 16, 64),
     (20, 1, 2, 1, 256, 256)])
