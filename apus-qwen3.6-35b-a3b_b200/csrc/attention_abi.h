@@ -93,8 +93,8 @@ extern "C" int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t 
                                        size_t rows, void *stream) {
     KvView v;
     if (kv_view(kv, "kv_extend_dev", &v)) return 1;
-    if (!n) return 0;
-    if (!d_cu || n > kv->seqs || (d_slot && rows > 0x7fffffff))
+    if (!n && (!d_slot || !rows)) return 0;       /* (without a list no row has a place) */
+    if ((n && !d_cu) || n > kv->seqs || (d_slot && rows > 0x7fffffff))
         return fail("kv_extend_dev: bad args");
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;

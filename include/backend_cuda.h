@@ -591,8 +591,8 @@ typedef struct {
  * taking the lowest free pages in the order of the list; the tokens' keys and values are for
  * the caller to write (apus_cuda_rope_dev).  d_slot [rows] (optional): the place of packed row t
  * of d_cu, page * page_tokens + offset; -1 for rows outside of [d_cu[0], d_cu[n]) and for all
- * rows where the call is refused (pages run out, a sequence twice in the list or longer than
- * max_pages). */
+ * rows where the list is empty (n is 0; d_cu is not read then) or the call is refused (pages run
+ * out, a sequence twice in the list or longer than max_pages). */
 int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t *d_seq, const int32_t *d_cu,
                             size_t n, int32_t *d_slot, size_t rows, void *stream);
 /* Sequences d_dst[i] (empty, none twice, none a source as well) become copies of d_src[i]: full

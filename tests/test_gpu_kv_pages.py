@@ -431,3 +431,28 @@ def test_serving_run(gpu):
     live = int((cache.refs > 0).sum())
     gpu.kv_compact_dev(cache.c, stream=st)
     assert (cache.refs[:live] > 0).all() and (cache.refs[live:] == 0).all()
+
+
+def test_places_of_an_empty_list(gpu):
+    """A step whose list is empty: no row has a place, whatever the step before has left there, and
+    positions and cache that are run on these places all the same write nothing."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    cache = u.Cache(1, 9, 1, 16, 64, 3, 4).hold([20, 5, 0])
+    k0, v0, before = cache.k.clone(), cache.v.clone(), cache.state()
+    seq, cu = u.ints([0, 1]), u.ints([0, 2, 3])
+    for ds, dc in ((seq.data_ptr(), cu.data_ptr()), (None, cu.data_ptr()), (None, None)):
+        slot = u.ints([p * 16 + 2 for p in range(5)] + [-7])
+        gpu.kv_extend_dev(cache.c, ds, dc, 0, slot.data_ptr(), 5, stream=u.stream())
+        assert slot.tolist() == [-1] * 5 + [-7]
+    x = u.normal(5, 3, 64)
+    q, pos = torch.zeros(5, 1, 64, dtype=torch.bfloat16, device="cuda"), u.ints([range(5)])
+    r = B.Rope(q=x.data_ptr(), k=x[:, 1:].data_ptr(), v=x[:, 2:].data_ptr(), q_out=q.data_ptr(),
+               q_stride=192, k_stride=192, v_stride=192, rows=5, heads=1, kv_heads=1, head_dim=64,
+               rot_dim=64, pos=pos.data_ptr(), axes=1, sections=(32,), theta=1e4)
+    gpu.rope_dev(r, cache.c, 0, slot.data_ptr(), stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 0
+    for a, b in zip(before + [k0, v0], cache.state() + [cache.k, cache.v]):
+        assert torch.equal(a, b)
