@@ -193,6 +193,7 @@ __device__ __forceinline__ void ad_finish4(const AttnView &a, long row, int head
         y.z *= ad_gate(bf16lo(gate.y));
         y.w *= ad_gate(bf16hi(gate.y));
     }
+    if (sum == 0.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);     /* no key, whatever the gate is */
     *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + head * D + c) =
         make_uint2(pack_bf16_rn(y.x, y.y), pack_bf16_rn(y.z, y.w));
     if (c == 0 && a.lse)
@@ -558,8 +559,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                           y1 = o[n][k >> 1][(k & 1) * 2 + 1] * v1;
                     if (p.a.gate) {
                         const uint32_t x = ad_transpose(gt[k]);
-                        y0 *= ad_gate(bf16lo(x));
-                        y1 *= ad_gate(bf16hi(x));
+                        /* (no key: zero, whatever the gate is) */
+                        y0 = v0 == 0.0f ? 0.0f : y0 * ad_gate(bf16lo(x));
+                        y1 = v1 == 0.0f ? 0.0f : y1 * ad_gate(bf16hi(x));
                     }
                     const uint32_t y = ad_transpose(pack_bf16_rn(y0, y1));
                     if (there)

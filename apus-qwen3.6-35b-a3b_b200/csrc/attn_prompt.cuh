@@ -856,6 +856,7 @@ __global__ void __launch_bounds__(256) attn_prompt_join_kernel(const __grid_cons
                 a *= ad_gate(bf16lo(z));
                 b *= ad_gate(bf16hi(z));
             }
+            if (sum == 0.0f) a = b = 0.0f;   /* no key, whatever the gate is */
             *reinterpret_cast<uint32_t *>(p.a.out + token * p.a.out_stride + at + i) =
                 pack_bf16_rn(a, b);
         }

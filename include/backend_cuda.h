@@ -635,7 +635,8 @@ int apus_cuda_rope_dev(const ApusCudaRope *r, const ApusCudaKvCache *kv, size_t 
 /* What both forms of attention take: s_j = scale q . k_j over the keys that a row sees,
  * p = softmax(s), out = (sum_j p_j v_j) * sigmoid(gate), narrowed once; lse = log sum_j exp(s_j).
  * Sums and statistics are fp32 (|s_j| below 2^30); p is narrowed to BF16 for its product
- * with v.  A row that sees no key gets zeros and -inf.  out overlaps no input. */
+ * with v.  A row that sees no key gets zeros and -inf, whatever its gate is.  out overlaps no
+ * input. */
 typedef struct {
     const uint16_t *q;                /* [rows][heads][head_dim] */
     const uint16_t *gate;             /* the same, or NULL: no gate */

@@ -451,3 +451,74 @@ def test_a_step_in_a_graph(gpu):
     for x, y in zip(one["c"].state() + [one["out"], one["c"].k, one["c"].v],
                     two["c"].state() + [two["out"], two["c"].k, two["c"].v]):
         assert torch.equal(x, y)
+
+
+def _no_key(out, lse):
+    return bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 2, 128), (16, 1, 64)])
+@pytest.mark.parametrize("nq,nk,launches", [([7, 2], [0, 3001], 2), ([40, 1], [30, 4000], 2),
+                                            ([200, 3], [150, 3], 1), ([90], [0], 1)])
+def test_prompt_rows_without_keys_beside_a_gate_that_is_not_finite(gpu, heads, kv_heads, dim, nq,
+                                                                   nk, launches):
+    """Zeros and -inf whatever the gate is, with shared keys and without."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    rows, keys = sum(nq), sum(nk)
+    q, g = u.normal(rows, 2, heads, dim, seed=1).unbind(1)
+    k, v = u.normal(keys + 1, 2, kv_heads, dim, seed=2).unbind(1)
+    blind = max(0, nq[0] - nk[0])            # the first sequence's first rows
+    for i, x in enumerate((math.nan, math.inf, -math.inf)):
+        g[i:blind:3] = x
+    out, lse = torch.full_like(q, 7.0).contiguous(), torch.full((rows, heads), 7.0, device="cuda")
+    cq, ck = u.ints(u.bounds(nq)), u.ints(u.bounds(nk))
+    a = u.attn(q, out, lse, g, kv_heads=kv_heads)
+    before = gpu.launches()
+    gpu.attn_prompt_dev(a, B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), k_stride=k.stride(0),
+                                      v_stride=v.stride(0), rows=keys, cu_q=cq.data_ptr(),
+                                      cu_k=ck.data_ptr(), seqs=len(nq), causal=1),
+                        stream=u.stream())
+    torch.cuda.synchronize()
+    assert gpu.launches() - before == launches
+    assert _no_key(out[:blind], lse[:blind])
+    at = 0
+    for i, (n, m) in enumerate(zip(nq, nk)):
+        s = slice(at + max(0, n - m), at + n)
+        limit = m - (s.stop - s.start) + 1 + torch.arange(s.stop - s.start, device="cuda")
+        ks = slice(sum(nk[:i]), sum(nk[:i + 1]))
+        if s.stop > s.start:
+            u.check(out[s], lse[s], u.exact(q[s], k[ks], v[ks], limit, a.scale, g[s]))
+        at += n
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (8, 2, 128), (16, 1, 64)])
+@pytest.mark.parametrize("lengths", [[10, 40], [20, 33], [3000, 50], [700] + [9] * 150,
+                                     [9] + [1500] * 64, [9000] + [16] * 20])
+def test_decode_rows_without_a_page_beside_a_gate_that_is_not_finite(gpu, heads, kv_heads, dim,
+                                                                     lengths):
+    """All page numbers of a sequence outside of the pool: zeros and -inf whatever the gate is, where one
+    warp, one SM and several of them sum such a row up; the others are what they would be."""
+    import torch
+    import attn_util as u
+    page, n = 16, len(lengths)
+    held = [-(-m // page) for m in lengths]
+    cache = u.Cache(1, sum(held) + 1, kv_heads, page, dim, n, max(held) + 1).hold(lengths)
+    bad = [0] + list(range(3, n, 5))
+    for s in bad:
+        cache.table[s] = cache.pages + s
+    q, g = u.normal(n, 2, heads, dim, seed=3).unbind(1)
+    for i, s in enumerate(bad):
+        g[s] = (math.nan, math.inf, -math.inf)[i % 3]
+    out, lse = torch.full_like(q, 7.0).contiguous(), torch.full((n, heads), 7.0, device="cuda")
+    a = u.attn(q, out, lse, g, kv_heads=kv_heads)
+    gpu.attn_decode_dev(a, cache.c, 0, None, stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 3
+    assert _no_key(out[bad], lse[bad])
+    for s in (1, 2, n - 1):
+        if s < n and s not in bad:
+            k, v = cache.tokens(0, s)
+            u.check(out[s:s + 1], lse[s:s + 1], u.exact(q[s:s + 1], k, v, u.ints([lengths[s]]),
+                                                        a.scale, g[s:s + 1]))
