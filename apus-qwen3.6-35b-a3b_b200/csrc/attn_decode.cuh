@@ -199,18 +199,20 @@ __device__ __forceinline__ void ad_finish4(const AttnView &a, long row, int head
     if (c == 0 && a.lse)
         a.lse[row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
+/* Two such words.  Of a vector access each element is whole, not the vector: a value and its round
+ * are the halves of one 64-bit element, so that none is seen without the other. */
 __device__ __forceinline__ void ad_put2(uint2 *at, float x, float y, unsigned round) {
-    asm volatile("st.relaxed.gpu.global.v4.u32 [%0], {%1, %2, %3, %2};" ::"l"(at),
-                 "r"(__float_as_uint(x)), "r"(round), "r"(__float_as_uint(y))
+    const uint64_t tag = (uint64_t)round << 32;
+    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(at),
+                 "l"(tag | __float_as_uint(x)), "l"(tag | __float_as_uint(y))
                  : "memory");
 }
 __device__ __forceinline__ uint4 ad_look2(const uint2 *at) {
-    uint4 v;
-    asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+    uint64_t a, b;
+    asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b)
                  : "l"(at)
                  : "memory");
-    return v;
+    return make_uint4((uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32));
 }
 /* Four values and a head's max and sum, looked at once already: again until they are this
  * round's, for about a second at most. */

@@ -522,3 +522,40 @@ def test_decode_rows_without_a_page_beside_a_gate_that_is_not_finite(gpu, heads,
             k, v = cache.tokens(0, s)
             u.check(out[s:s + 1], lse[s:s + 1], u.exact(q[s:s + 1], k, v, u.ints([lengths[s]]),
                                                         a.scale, g[s:s + 1]))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(16, 2, 256, [977]), (8, 1, 128, [20011]),
+                                                        (6, 2, 64, [3000, 700, 41])])
+def test_parts_of_other_sms_are_of_this_call(gpu, heads, kv_heads, dim, lengths):
+    """Two queries in turns, many times with nothing between: every result has the bits that it has
+    alone, so no value of the call before passes as this one's."""
+    import torch
+    import attn_util as u
+    n = len(lengths)
+    held = [-(-m // 32) for m in lengths]
+    cache = u.Cache(1, sum(held) + 1, kv_heads, 32, dim, n, max(held) + 1).hold(lengths)
+    qs = [u.normal(n, heads, dim, seed=s) for s in (1, 2)]
+    outs = [torch.empty_like(q) for q in qs]
+    lses = [torch.empty(n, heads, device="cuda") for _ in qs]
+    calls = [u.attn(*t, kv_heads=kv_heads) for t in zip(qs, outs, lses)]
+    want = []
+    for c, o, l in zip(calls, outs, lses):
+        gpu.attn_decode_dev(c, cache.c, 0, None, stream=u.stream())
+        torch.cuda.synchronize()
+        want.append((o.clone(), l.clone()))
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(20):
+            for c in calls:
+                gpu.attn_decode_dev(c, cache.c, 0, None, stream=u.stream())
+        for (o, l), (p, m) in zip(zip(outs, lses), want):
+            wrong += (o != p).sum() + (l != m).sum()
+    for _ in range(100):
+        graph.replay()
+    for _ in range(200):
+        for c, o, l, (p, m) in zip(calls, outs, lses, want):
+            gpu.attn_decode_dev(c, cache.c, 0, None, stream=u.stream())
+            wrong += (o != p).sum() + (l != m).sum()
+    torch.cuda.synchronize()
+    assert int(wrong) == 0 and gpu.last_block_status() == 0
