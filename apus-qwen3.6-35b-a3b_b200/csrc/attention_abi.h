@@ -499,6 +499,7 @@ extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKv
     p.shared_parts = x->d_attn_parts;
     p.parts = reinterpret_cast<float *>(x->d_attn_parts +
                                         (size_t)x->sm_count * 2 * AD_SHARED_WORDS);
+    p.blocks = x->sm_count;
     p.sync = x->d_attn_sync;
     const bool wide = p.a.group > 8;
     if (D == 64) return wide ? launch_decode<64, 16>(x, mk, mv, p, st)
@@ -507,4 +508,14 @@ extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKv
                               : launch_decode<128, 8>(x, mk, mv, p, st);
     return wide ? launch_decode<256, 16>(x, mk, mv, p, st)
                 : launch_decode<256, 8>(x, mk, mv, p, st);
+}
+
+extern "C" int apus_cuda_debug_attn_rounds(uint32_t rounds) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    DeviceGuard dev(g_ctx->device);
+    CU_OK(cudaDeviceSynchronize());
+    CU_OK(cudaMemcpy(g_ctx->d_attn_sync + AD_SYNC_ROUND, &rounds, sizeof rounds,
+                     cudaMemcpyHostToDevice));
+    return 0;
 }

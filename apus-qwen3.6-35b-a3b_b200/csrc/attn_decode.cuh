@@ -28,6 +28,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "attn_tags.h"
 #include "attn_view.cuh"
 #include "common.cuh"
 #include "kv_pages.cuh"
@@ -58,12 +59,13 @@ struct DecodeParams {
     int row0, rows;                          /* of this launch */
     uint2 *shared_parts;                     /* [gridDim][2]: began in an earlier CTA, or here */
     float *parts;                            /* [gridDim][warps]: ends in the warp, began before it */
-    unsigned *sync;                          /* rounds so far, CTAs that have seen the number */
+    int blocks;                              /* CTAs that shared_parts has room for */
+    unsigned *sync;                          /* the last round, CTAs that have seen its number */
 };
 
 /* a part as other SMs read it: every float beside the number of the round that wrote it, so that
  * it is its own flag (no fence, no second look): (value, round) words, outputs and then a
- * head's max and sum side by side */
+ * head's max and sum side by side (attn_tags.h: how a number comes again) */
 constexpr int AD_SHARED_ML = AD_MAX_GROUP * AD_MAX_DIM;
 constexpr int AD_SHARED_WORDS = AD_SHARED_ML + 2 * AD_MAX_GROUP;
 inline size_t ad_scratch_bytes(int sms) {
@@ -255,7 +257,13 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     }
     pdl_enter();
     /* this round's number: no word holds it yet */
-    const unsigned round = *reinterpret_cast<volatile unsigned *>(p.sync + AD_SYNC_ROUND) + 1;
+    const unsigned round =
+        ad_round_after(*reinterpret_cast<volatile unsigned *>(p.sync + AD_SYNC_ROUND));
+    /* (this CTA's own words, before it writes any, and those of CTAs that there are not) */
+    if (ad_round_clears(round))
+        for (int b = blockIdx.x; b < p.blocks; b += gridDim.x)
+            for (int i = tid; i < AD_SHARED_WORDS; i += AD_THREADS)
+                ad_put2(p.shared_parts + (size_t)b * 2 * AD_SHARED_WORDS + 2 * i, 0.0f, 0.0f, 0);
 
     /* ---- the line: tiles before every row (each CTA for itself) ---- */
     {
@@ -760,7 +768,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             if (real && sub == 0) ad_finish4(p.a, row, head, D, c, acc, top, sum, gate);
         }
     }
-    if (tid == 0 && seen == gridDim.x - 1) atomicAdd(p.sync + AD_SYNC_ROUND, 1u);
+    if (tid == 0 && seen == gridDim.x - 1) atomicExch(p.sync + AD_SYNC_ROUND, round);
 }
 
 }  // namespace apus

@@ -671,6 +671,10 @@ int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *key
  * block. */
 int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv, size_t layer,
                               const int32_t *d_seq, void *stream);
+/* Diagnostic of it (synchronous): its round counter as after this many launches, of a turn of
+ * 2^32 - 1, so that a test can see it wrap.  To be set ahead only, or behind a clearing round
+ * (csrc/attn_tags.h) that has been run. */
+int apus_cuda_debug_attn_rounds(uint32_t rounds);
 
 /* ---- synthetic tensors (benchmarks and tests) ---------------------------- */
 /* Fill n BF16 elements with the counter-based approximately-normal stream

@@ -559,3 +559,54 @@ def test_parts_of_other_sms_are_of_this_call(gpu, heads, kv_heads, dim, lengths)
             wrong += (o != p).sum() + (l != m).sum()
     torch.cuda.synchronize()
     assert int(wrong) == 0 and gpu.last_block_status() == 0
+
+
+def test_decode_at_the_end_of_the_round_counter(gpu):
+    """Words of parts that go from SM to SM carry their round, and the counter wraps: neither words
+    that nobody has written nor those of a turn ago pass as this call's."""
+    import torch
+    import attn_util as u
+    END = (1 << 32) - 1
+    runs = []
+    for lengths, kv_heads, seed in (([9000, 700], 2, 1), ([977], 2, 2), ([20], 1, 3)):
+        held = [-(-m // 32) for m in lengths]
+        cache = u.Cache(1, sum(held), kv_heads, 32, 128, len(lengths), max(held)).hold(lengths)
+        q = u.normal(len(lengths), 8 * kv_heads, 128, seed=seed)
+        out = torch.empty_like(q)
+        runs.append((u.attn(q, out, kv_heads=kv_heads), cache, q, out))
+
+    def run(i):
+        a, cache, _, out = runs[i]
+        out.fill_(7.0)
+        gpu.attn_decode_dev(a, cache.c, 0, None, stream=u.stream())
+        torch.cuda.synchronize()
+        assert gpu.last_block_status() == 0
+        return out.clone()
+
+    gpu.debug_attn_rounds(END - 2)                # nothing has been written yet
+    early = [run(0) for _ in range(6)]
+    gpu.disable()
+    gpu.enable()
+    want = [run(i) for i in range(3)]
+    k, v = runs[0][1].tokens(0, 0)
+    u.check(want[0][:1], None, u.exact(runs[0][2][:1], k, v, u.ints([9000]), 128 ** -0.5))
+    assert all(torch.equal(x, want[0]) for x in early)
+    for clearing in (0x40000000, 0xbfffffff):
+        gpu.debug_attn_rounds(1000)
+        old = runs[0][2].clone()
+        runs[0][2].copy_(-old)
+        assert not torch.equal(run(0), want[0])   # words of rounds 1001 to 1004
+        run(0), run(0), run(0)
+        runs[0][2].copy_(old)
+        gpu.debug_attn_rounds(clearing - 2)       # one CTA, which clears the words of all
+        for _ in range(4):
+            assert torch.equal(run(2), want[2])
+        gpu.debug_attn_rounds(1000)
+        for i in (0, 1, 0, 0):
+            assert torch.equal(run(i), want[i])
+        gpu.debug_attn_rounds(clearing - 3)       # and launches that clear and sum up
+        for i in (0, 1, 0, 0, 1, 0):
+            assert torch.equal(run(i), want[i])
+    gpu.debug_attn_rounds(END - 3)
+    for i in (0, 1, 0, 0, 1, 2, 0):
+        assert torch.equal(run(i), want[i])
