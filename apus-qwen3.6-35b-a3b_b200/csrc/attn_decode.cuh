@@ -216,6 +216,12 @@ __device__ __forceinline__ uint4 ad_look2(const uint2 *at) {
                  : "memory");
     return make_uint4((uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32));
 }
+/* A copy's barrier by a whole warp, with one answer: lanes that went on alone would wait for the others
+ * in the next shuffle or MMA for good. */
+__device__ __forceinline__ bool ad_wait(uint64_t *bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+}
 /* Four values and a head's max and sum, looked at once already: again until they are this
  * round's, for about a second at most. */
 __device__ __forceinline__ bool ad_get(const uint2 *at, const uint2 *at_ml, unsigned round,
@@ -427,7 +433,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     while (alive && done < to) {
         /* ---- scores of 16 tokens ---- */
         int st = (int)(used % STAGES);
-        if (!mbar_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
+        if (!ad_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
             alive = false;
             break;
         }
@@ -502,7 +508,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
         }
         /* ---- outputs ---- */
         st = (int)(used % STAGES);
-        if (!mbar_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
+        if (!ad_wait(&s.full[warp][st], (used / STAGES) & 1u)) {
             alive = false;
             break;
         }
