@@ -119,7 +119,8 @@ SYMBOLS = [
     "apus_cuda_resadd_dev", "apus_cuda_bf16_gemv_dev", "apus_cuda_kv_extend_dev",
     "apus_cuda_kv_fork_dev", "apus_cuda_kv_free_dev", "apus_cuda_kv_compact_dev",
     "apus_cuda_kv_copy_dev", "apus_cuda_rope_dev", "apus_cuda_attn_prompt_dev",
-    "apus_cuda_attn_decode_dev", "apus_cuda_debug_attn_rounds", "apus_synth_fill_host",
+    "apus_cuda_attn_decode_dev", "apus_cuda_debug_attn_rounds", "apus_cuda_debug_attn_absent",
+    "apus_synth_fill_host",
     "apus_synth_fill_dev",
 ]
 
@@ -224,6 +225,7 @@ class Backend:
         L.apus_cuda_attn_prompt_dev.argtypes = [C.POINTER(Attn), C.POINTER(AttnKeys), vp]
         L.apus_cuda_attn_decode_dev.argtypes = [C.POINTER(Attn), kv, sz, vp, vp]
         L.apus_cuda_debug_attn_rounds.argtypes = [C.c_uint32]
+        L.apus_cuda_debug_attn_absent.argtypes = [C.c_int]
         L.apus_synth_fill_host.argtypes = [u16p, sz, C.c_uint64, C.c_uint32,
                                            C.c_uint32, C.c_uint64, C.c_double]
         L.apus_synth_fill_host.restype = None
@@ -688,6 +690,10 @@ class Backend:
     def debug_attn_rounds(self, rounds):
         """The round counter of attn_decode_dev as after this many launches (tests only)"""
         self._check(self.lib.apus_cuda_debug_attn_rounds(rounds), "apus_cuda_debug_attn_rounds")
+
+    def debug_attn_absent(self, cta):
+        """In the next attention call this CTA loads nothing (tests only)"""
+        self._check(self.lib.apus_cuda_debug_attn_absent(cta), "apus_cuda_debug_attn_absent")
 
     # ---- synthetic tensors -------------------------------------------------------
     def synth_fill_host(self, n, seed, layer, tensor_id, sigma, first=0):

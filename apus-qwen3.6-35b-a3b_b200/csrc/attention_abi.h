@@ -421,6 +421,8 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     p.parts = c->d_attn_split;
     p.sched = c->d_attn_sync + AD_SYNC_WORDS;
     p.status = c->d_status;
+    p.absent = c->attn_absent;
+    c->attn_absent = -1;
     if (a->head_dim == 64) return launch_prompt<64>(c, p, keys, k_stride, v_stride, st);
     if (a->head_dim == 128) return launch_prompt<128>(c, p, keys, k_stride, v_stride, st);
     return launch_prompt<256>(c, p, keys, k_stride, v_stride, st);
@@ -500,6 +502,8 @@ extern "C" int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKv
     p.parts = reinterpret_cast<float *>(x->d_attn_parts +
                                         (size_t)x->sm_count * 2 * AD_SHARED_WORDS);
     p.blocks = x->sm_count;
+    p.absent = x->attn_absent;
+    x->attn_absent = -1;
     p.sync = x->d_attn_sync;
     const bool wide = p.a.group > 8;
     if (D == 64) return wide ? launch_decode<64, 16>(x, mk, mv, p, st)
@@ -517,5 +521,11 @@ extern "C" int apus_cuda_debug_attn_rounds(uint32_t rounds) {
     CU_OK(cudaDeviceSynchronize());
     CU_OK(cudaMemcpy(g_ctx->d_attn_sync + AD_SYNC_ROUND, &rounds, sizeof rounds,
                      cudaMemcpyHostToDevice));
+    return 0;
+}
+extern "C" int apus_cuda_debug_attn_absent(int cta) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (ctx_init()) return 1;
+    g_ctx->attn_absent = cta;
     return 0;
 }

@@ -57,6 +57,7 @@ struct DecodeParams {
     int *wait_status;                        /* the library's */
     int pages, page_tokens, page_tiles, seqs, max_pages, kv_heads;
     int row0, rows;                          /* of this launch */
+    int absent;                              /* a CTA that asks for no tile (a test's), or -1 */
     uint2 *shared_parts;                     /* [gridDim][2]: began in an earlier CTA, or here */
     float *parts;                            /* [gridDim][warps]: ends in the warp, began before it */
     int blocks;                              /* CTAs that shared_parts has room for */
@@ -223,10 +224,10 @@ __device__ __forceinline__ bool ad_wait(uint64_t *bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
 }
 /* Four values and a head's max and sum, looked at once already: again until they are this
- * round's, for about a second at most. */
+ * round's, for about a second at most (a look is an L2 round trip, four times a barrier's). */
 __device__ __forceinline__ bool ad_get(const uint2 *at, const uint2 *at_ml, unsigned round,
                                        uint4 &a, uint4 &b, uint4 &ml) {
-    for (uint32_t i = 0; i < APUS_WAIT_LIMIT; i++) {
+    for (uint32_t i = 0; i < APUS_WAIT_LIMIT / 4; i++) {
         if (a.y == round && a.w == round && b.y == round && b.w == round && ml.y == round &&
             ml.w == round)
             return true;
@@ -368,7 +369,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
             coord = (page * p.kv_heads + ci.head) * p.page_tokens +
                     (int)((unsigned)ci.tile % (unsigned)p.page_tiles) * AD_TILE;
         }
-        if (lane == 0) {
+        if (lane == 0 && (int)blockIdx.x != p.absent) {
             s.valid[warp][st] = count;
             mbar_expect_tx(&s.full[warp][st], TILE_BYTES);
             tma_load_3d(ring + st * TILE_BYTES, keys ? &map_k : &map_v, 0, coord, 0,
@@ -604,8 +605,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k,
     }
     if (!alive) {                                         /* a copy never came: no result, no hang */
         if (lane == 0) set_status(p.wait_status, ST_MBAR_TIMEOUT);
-        for (; used < copies; used++)
-            mbar_wait(&s.full[warp][used % STAGES], (used / STAGES) & 1u);
+        /* what is under way lands before the CTA leaves (one more limit, not one for each) */
+        while (used < copies && ad_wait(&s.full[warp][used % STAGES], (used / STAGES) & 1u)) used++;
     }
     __syncthreads();                                      /* every ring is read to its end */
 

@@ -81,6 +81,7 @@ struct PromptParams {
     int splits;                              /* CTAs that share a tile's keys */
     float *parts;                            /* with splits: [items][AP_PART_FLOATS] */
     unsigned *sched;                         /* next item; [32]: CTAs that are through */
+    int absent;                              /* a CTA that loads three pieces (a test's), or -1 */
     int *status;
 };
 
@@ -373,7 +374,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
         auto load = [&](bool keys, const ApItem &t, int j) {
             for (int u = 0; u < S::UNITS && alive; u++, unit++) {
                 const int st = (int)(unit % STAGES);
-                if (!pg_wait(&s.kv_empty[st], ((unit / STAGES) & 1u) ^ 1u, abort_flag, p.status,
+                if ((unit == 3 && (int)blockIdx.x == p.absent) ||
+                    !pg_wait(&s.kv_empty[st], ((unit / STAGES) & 1u) ^ 1u, abort_flag, p.status,
                              ST_MBAR_TIMEOUT)) {
                     alive = false;
                     return;

@@ -135,6 +135,7 @@ struct Ctx {
     uint2 *d_attn_parts = nullptr;
     unsigned *d_attn_sync = nullptr;
     float *d_attn_split = nullptr;       /* [sm_count][AP_PART_FLOATS] */
+    int attn_absent = -1;                /* a CTA that gives up in the next call (a test's) */
     size_t df_act_elems = 0, df_sa_elems = 0;
     int last_block_launches = 0;
     int last_block_path = 0;

@@ -147,14 +147,21 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 /* Bounded wait: about a second at most, then give up.  Returns false on
- * timeout (the caller records a status code and unwinds). */
+ * timeout (the caller records a status code and unwinds).  A try that fails has been suspended for
+ * some 4 us before it says so (2^22 of them took 17 s), so behind the first ones a barrier is only
+ * looked at, and the sleep between is what a turn takes. */
 #ifndef APUS_WAIT_LIMIT
 #define APUS_WAIT_LIMIT (1u << 22)
 #endif
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
     for (uint32_t i = 0; i < APUS_WAIT_LIMIT; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (i > 64) __nanosleep(64);
+        if (i <= 64) {
+            if (mbar_try_wait(bar, parity)) return true;
+        } else {
+            if (mbar_test(bar, parity)) return true;
+            __nanosleep(64);
+        }
     }
     return false;
 }

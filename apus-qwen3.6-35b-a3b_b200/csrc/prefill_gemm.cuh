@@ -181,9 +181,12 @@ __device__ __forceinline__ bool pg_wait(uint64_t *bar, uint32_t parity,
                                         int code) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
+#pragma unroll 1
     for (uint32_t i = 0; i < APUS_WAIT_LIMIT; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (i > 256) {
+        if (i <= 256) {
+            if (mbar_try_wait(bar, parity)) return true;
+        } else {                             /* (a try takes 4 us, 2^22 of them 17 s) */
+            if (mbar_test(bar, parity)) return true;
             __nanosleep(32);
             if (*abort_flag) return false;
         }

@@ -653,7 +653,8 @@ typedef struct {
  * none.  Rows of out and lse outside of [cu_q[0], cu_q[seqs]) stay as they are.  No value of
  * another sequence, or of a key behind the last one that a tile of rows may see, reaches a row,
  * whatever it is.  (Among the tokens of one such tile, at most 128 rows of one key head, a
- * value that is not finite spreads, as it does in a matrix product with zeros.) */
+ * value that is not finite spreads, as it does in a matrix product with zeros.)  A wait inside that
+ * runs out: apus_cuda_last_block_status(), as for the block. */
 typedef struct {
     const uint16_t *k, *v;            /* [rows][kv_heads][head_dim] */
     const int32_t *cu_q, *cu_k;       /* [seqs + 1] */
@@ -675,6 +676,12 @@ int apus_cuda_attn_decode_dev(const ApusCudaAttn *a, const ApusCudaKvCache *kv, 
  * 2^32 - 1, so that a test can see it wrap.  To be set ahead only, or behind a clearing round
  * (csrc/attn_tags.h) that has been run. */
 int apus_cuda_debug_attn_rounds(uint32_t rounds);
+/* ... and of what both forms of attention do when something never comes: in the next call this CTA
+ * asks for no keys (one token), or for no more than the first three pieces of them (prompts).  The
+ * waits run out, a limit of about a second each (one token: its own, that for copies under way, the
+ * other CTAs' for its parts), the status is 1, 2 or 4, the results are not valid, and later calls are
+ * as ever. */
+int apus_cuda_debug_attn_absent(int cta);
 
 /* ---- synthetic tensors (benchmarks and tests) ---------------------------- */
 /* Fill n BF16 elements with the counter-based approximately-normal stream

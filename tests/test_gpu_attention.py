@@ -610,3 +610,65 @@ def test_decode_at_the_end_of_the_round_counter(gpu):
     gpu.debug_attn_rounds(END - 3)
     for i in (0, 1, 0, 0, 1, 2, 0):
         assert torch.equal(run(i), want[i])
+
+
+def _with_a_cta_that_gives_up(gpu, torch, call, results, cta, codes):
+    import time
+    call()
+    torch.cuda.synchronize()
+    want = [r.clone() for r in results]
+    assert gpu.last_block_status() == 0
+    gpu.debug_attn_absent(cta)
+    t = time.monotonic()
+    call()
+    torch.cuda.synchronize()
+    took = time.monotonic() - t
+    assert gpu.last_block_status() in codes
+    assert took < 10, took                   # a few limits of about a second, not one for each copy
+    for _ in range(3):
+        for r in results:
+            r.fill_(7.0)
+        call()
+        torch.cuda.synchronize()
+        assert gpu.last_block_status() == 0
+        assert all(torch.equal(r, w) for r, w in zip(results, want))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths,cta", [
+    (16, 2, 256, [20011], 5), (8, 1, 128, [20011], 0), (12, 12, 64, [1500] * 64, 147),
+    (16, 1, 256, [700, 9000], 30), (6, 2, 64, [20], 0)])
+def test_decode_with_keys_that_never_come(gpu, heads, kv_heads, dim, lengths, cta):
+    """A CTA that asks for no keys: its waits for them and the others' for its parts run out, the
+    status says so, and the next calls are right."""
+    import torch
+    import attn_util as u
+    n = len(lengths)
+    held = [-(-m // 32) for m in lengths]
+    cache = u.Cache(1, sum(held), kv_heads, 32, dim, n, max(held)).hold(lengths)
+    q = u.normal(n, heads, dim, seed=1)
+    out, lse = torch.empty_like(q), torch.empty(n, heads, device="cuda")
+    a = u.attn(q, out, lse, kv_heads=kv_heads)
+    _with_a_cta_that_gives_up(gpu, torch, lambda: gpu.attn_decode_dev(
+        a, cache.c, 0, None, stream=u.stream()), [out, lse], cta, (1, 4))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,nq,nk,cta", [
+    (16, 2, 256, [900, 70], [900, 70], 3), (32, 8, 128, [3000], [3000], 100),
+    (8, 2, 64, [700], [700], 0), (16, 2, 256, [20], [9000], 7), (16, 2, 256, [77], [77], 1),
+    (12, 12, 64, [33], [5000], 0)])
+def test_prompt_with_keys_that_never_come(gpu, heads, kv_heads, dim, nq, nk, cta):
+    """A CTA whose loads end in the middle of a tile: no MMA, load or wait outlives it, the status
+    says so, and the next calls are right."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    q, g = u.normal(sum(nq), 2, heads, dim, seed=1).unbind(1)
+    k, v = u.normal(sum(nk), 2, kv_heads, dim, seed=2).unbind(1)
+    out = torch.empty(sum(nq), heads, dim, dtype=torch.bfloat16, device="cuda")
+    lse = torch.empty(sum(nq), heads, device="cuda")
+    cq, ck = u.ints(u.bounds(nq)), u.ints(u.bounds(nk))
+    a = u.attn(q, out, lse, g, kv_heads=kv_heads)
+    kk = B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), k_stride=k.stride(0), v_stride=v.stride(0),
+                    rows=sum(nk), cu_q=cq.data_ptr(), cu_k=ck.data_ptr(), seqs=len(nq), causal=1)
+    _with_a_cta_that_gives_up(gpu, torch, lambda: gpu.attn_prompt_dev(a, kk, stream=u.stream()),
+                              [out, lse], cta, (2,))
