@@ -82,7 +82,8 @@ class Attn(C.Structure):
 class AttnKeys(C.Structure):
     """ApusCudaAttnKeys"""
     _fields_ = [(k, vp) for k in ("k", "v", "cu_q", "cu_k")] + \
-        [(k, sz) for k in ("k_stride", "v_stride", "rows", "seqs")] + [("causal", C.c_int)]
+        [(k, sz) for k in ("k_stride", "v_stride", "rows", "seqs")] + \
+        [("causal", C.c_int), ("longest", C.c_uint32)]
 
 
 # every symbol include/backend_cuda.h declares

@@ -399,7 +399,6 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     if (slots * a->kv_heads > (1u << 30)) return fail("attn_prompt_dev: too many rows");
     p.slots = (int)slots;
     p.items = (int)(slots * a->kv_heads);
-    const size_t steps = (keys->rows + AP_ROWS - 1) / AP_ROWS;     /* of a tile, at most */
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
     Ctx *c = g_ctx;
@@ -411,7 +410,13 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
      * takes as long as two or three.  head_dim 256, 2 key heads: 16 rows over 4096 keys 52 -> 31
      * us, 128 rows over 30128 331 -> 77, one row over 1000 20 -> 17.  Where the parts would fill
      * the SMs, their way through memory takes longer than a few steps: 400 rows over 1000 keys 21
-     * -> 26, so only from sixteen steps on. */
+     * -> 26, so only from sixteen steps on.
+     * How many steps a tile has is on the device; the caller may say how many keys the longest
+     * sequence has.  Else all of them count, which one sequence may hold nearly alone: a row over 4000
+     * beside seven over 50 would take 49 us by the mean, and takes 19.  Where they are even, parts are short
+     * or empty without that number: eight rows over 200 keys each 14.3 us, 9.5 with it. */
+    const size_t most = keys->longest && keys->longest < keys->rows ? keys->longest : keys->rows;
+    const size_t steps = (most + AP_ROWS - 1) / AP_ROWS;
     size_t splits = (size_t)c->sm_count / p.items;
     if (splits > steps / 4) splits = steps / 4;
     if (splits > AP_MAX_SPLITS) splits = AP_MAX_SPLITS;

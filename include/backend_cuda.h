@@ -660,6 +660,8 @@ typedef struct {
     const int32_t *cu_q, *cu_k;       /* [seqs + 1] */
     size_t k_stride, v_stride, rows, seqs;
     int causal;
+    uint32_t longest;                 /* keys of the longest sequence; 0: not known, up to all rows
+                                       * (for speed alone: how many CTAs share a tile's keys) */
 } ApusCudaAttnKeys;
 int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAttnKeys *keys, void *stream);
 

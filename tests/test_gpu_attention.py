@@ -672,3 +672,34 @@ def test_prompt_with_keys_that_never_come(gpu, heads, kv_heads, dim, nq, nk, cta
                     rows=sum(nk), cu_q=cq.data_ptr(), cu_k=ck.data_ptr(), seqs=len(nq), causal=1)
     _with_a_cta_that_gives_up(gpu, torch, lambda: gpu.attn_prompt_dev(a, kk, stream=u.stream()),
                               [out, lse], cta, (2,))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (32, 8, 128), (8, 2, 64)])
+def test_prompt_short_sequences_do_not_share_keys(gpu, heads, kv_heads, dim):
+    """Where the caller says how long the longest sequence is, keys are shared only if a tile has
+    enough of them for two CTAs, however many they are together.  A number that is too small or too
+    large changes nothing of the result but the order of its sums."""
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    for nq, nk, longest, launches in (([1] * 8, [200] * 8, 200, 1), ([5, 40], [133, 870], 870, 1),
+                                      ([5, 40], [133, 900], 900, 2),        # (eight steps)
+                                      ([1], [1600], 1600, 2), ([1], [1600], 0, 2),
+                                      ([1, 1], [2000, 3], 2000, 2), ([1, 1], [2000, 3], 17, 1),
+                                      ([1, 1], [2000, 3], 0xffffffff, 2)):
+        q, k, v = (u.normal(sum(n), h, dim, seed=i) for i, (n, h) in
+                   enumerate(((nq, heads), (nk, kv_heads), (nk, kv_heads))))
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        cq, ck = u.bounds(nq), u.bounds(nk)
+        dq, dk = u.ints(cq), u.ints(ck)
+        a = u.attn(q, out, lse, kv_heads=kv_heads)
+        before = gpu.launches()
+        gpu.attn_prompt_dev(a, B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=sum(nk),
+                                          cu_q=dq.data_ptr(), cu_k=dk.data_ptr(), seqs=len(nq),
+                                          causal=1, longest=longest), stream=u.stream())
+        torch.cuda.synchronize()
+        assert gpu.launches() - before == launches, (nk, longest)
+        for i in range(len(nq)):
+            qs, ks = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
+            limit = nk[i] - nq[i] + 1 + torch.arange(nq[i], device="cuda")
+            u.check(out[qs], lse[qs], u.exact(q[qs], k[ks], v[ks], limit, a.scale))
