@@ -456,3 +456,55 @@ def test_places_of_an_empty_list(gpu):
     assert cache.status() == 0
     for a, b in zip(before + [k0, v0], cache.state() + [cache.k, cache.v]):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("pages", [8193, 20000, 300001])
+def test_pools_of_more_pages_than_are_asked_for_ahead(gpu, pages):
+    """Pages taken, shared, given back and moved together all over a large pool, most of it held
+    by a user that is in no row of the table."""
+    import torch
+    import attn_util as u
+    seqs, page = 6, 16
+    cache = u.Cache(1, pages, 1, page, 64, seqs, 1200)
+    rng = np.random.default_rng(pages)
+    used = rng.random(pages) < 0.9
+    used[-40:] = False                                   # (the last warp's last piece, too)
+    cache.refs.copy_(torch.from_numpy(used.astype(np.int32)))
+    k0, v0, book, st = cache.k.clone(), cache.v.clone(), Book(cache), u.stream()
+
+    def extend(seq, add):
+        assert book.extend(seq, add)
+        ds, dc = u.ints(seq), u.ints(u.bounds(add))
+        slot = torch.zeros(sum(add), dtype=torch.int32, device="cuda")
+        start = [book.len[s] - a for s, a in zip(seq, add)]
+        gpu.kv_extend_dev(cache.c, ds.data_ptr(), dc.data_ptr(), len(seq), slot.data_ptr(),
+                          sum(add), stream=st)
+        assert slot.tolist() == [book.table[s][t // page] * page + t % page
+                                 for s, n, a in zip(seq, start, add) for t in range(n, n + a)]
+
+    free = pages - int(used.sum())
+    extend([4, 0, 2], [page * (free // 4), 5, page * (free // 3) + 1] if free < 3000 else
+           [page * 1199, 5, page * 1000 + 1])
+    book.check(cache, k0, v0)
+    assert book.fork([0, 2], [1, 3])
+    s, d = u.ints([0, 2]), u.ints([1, 3])
+    gpu.kv_fork_dev(cache.c, s.data_ptr(), d.data_ptr(), 2, stream=st)
+    book.check(cache, k0, v0)
+    extend([1, 5], [40, 77])
+    book.free([4])
+    gpu.kv_free_dev(cache.c, u.ints([4]).data_ptr(), 1, stream=st)
+    book.check(cache, k0, v0)
+    book.compact()
+    gpu.kv_compact_dev(cache.c, stream=st)
+    book.check(cache, k0, v0)
+    # one page more than there are: refused, and all as it was
+    want = book.refs.count(0) + 1
+    if want <= 1200:
+        cu, one = u.ints([0, want * page]), u.ints([4])
+        gpu.kv_extend_dev(cache.c, one.data_ptr(), cu.data_ptr(), 1, stream=st)
+        assert cache.status() == 1
+        cache.work[0] = 0
+        extend([4], [(want - 1) * page])
+        assert 0 not in book.refs
+    book.check(cache, k0, v0)
+    assert cache.status() == 0
