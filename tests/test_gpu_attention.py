@@ -703,3 +703,111 @@ def test_prompt_short_sequences_do_not_share_keys(gpu, heads, kv_heads, dim):
             qs, ks = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
             limit = nk[i] - nq[i] + 1 + torch.arange(nq[i], device="cuda")
             u.check(out[qs], lse[qs], u.exact(q[qs], k[ks], v[ks], limit, a.scale))
+
+
+def _counted(n, dim, turn):
+    """Which value of a head counts a token: those of 16 tokens the same one, and another pairing
+    of such tiles with each turn."""
+    import torch
+    tile = torch.arange(n, device="cuda") // 16
+    return (tile + turn * 37 * (tile // dim)) % dim
+
+
+def _check_counts(out, lse, limit, code, dim):
+    """Equal scores: a value is the share of its tokens, lse the logarithm of their number.  Counts
+    are exact in fp32 (weights of one, below 2^24); what is left are the division and the product, 2 and
+    1/2 steps of 2^-23, and the narrowing, 2^-8; and for log2 and the product with ln(2) a step of fp32
+    each, of values below 2^4: 2 * 2^-20 at most.  A tile of 16 tokens more or less is 16 of
+    the 16 * (tiles / dim + 1) that its value counts."""
+    import torch
+    hot = torch.nn.functional.one_hot(code, dim).double().cumsum(0)
+    for i, n in enumerate(limit):
+        want = hot[n - 1] / n
+        assert ((out[i].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want).all(), (i, n)
+        assert ((lse[i].double() - math.log(n)).abs() <= 2.0 ** -19).all(), (i, n)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("lengths", [[20011], [9000, 3], [1500] * 9 + [40, 16, 700], [130] * 90,
+                                     [5003, 17, 30000]])
+def test_decode_counts_every_tile_once(gpu, heads, kv_heads, dim, lengths):
+    import torch
+    import attn_util as u
+    page, n = 32, len(lengths)
+    held = [-(-m // page) for m in lengths]
+    cache = u.Cache(1, sum(held) + 1, kv_heads, page, dim, n, max(held) + 1).hold(lengths)
+    q = torch.zeros(n, heads, dim, dtype=torch.bfloat16, device="cuda")
+    for turn in (0, 1):
+        codes = [_counted(m, dim, turn) for m in lengths]
+        cache.v.fill_(math.nan)
+        for s, c in enumerate(codes):
+            t = torch.arange(lengths[s], device="cuda")
+            hot = torch.nn.functional.one_hot(c, dim).bfloat16()
+            cache.v[0].transpose(1, 2)[cache.table[s][t // page].long(), t % page] = \
+                hot[:, None].expand(-1, kv_heads, -1)
+        out, lse = torch.full_like(q, 7.0), torch.full((n, heads), 7.0, device="cuda")
+        gpu.attn_decode_dev(u.attn(q, out, lse, kv_heads=kv_heads), cache.c, 0, None,
+                            stream=u.stream())
+        torch.cuda.synchronize()
+        assert cache.status() == 0 and gpu.last_block_status() == 0
+        for s, c in enumerate(codes):
+            _check_counts(out[s:s + 1], lse[s:s + 1], [lengths[s]], c, dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("nq,nk,launches", [([1], [20011], 2), ([33], [5000], 2),
+                                            ([3, 9], [2000, 1800], 2), ([300], [3000], None),
+                                            ([700, 90], [700, 2500], None)])
+def test_prompt_counts_every_tile_once(gpu, heads, kv_heads, dim, nq, nk, launches):
+    import torch
+    import attn_util as u
+    import apus_b200.backend as B
+    q = torch.zeros(sum(nq), heads, dim, dtype=torch.bfloat16, device="cuda")
+    k = u.normal(sum(nk), kv_heads, dim)
+    cq, ck = u.bounds(nq), u.bounds(nk)
+    dq, dk = u.ints(cq), u.ints(ck)
+    for turn in (0, 1):
+        codes = [_counted(m, dim, turn) for m in nk]
+        v = torch.nn.functional.one_hot(torch.cat(codes), dim).bfloat16()[:, None].expand(
+            -1, kv_heads, -1).contiguous()
+        out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+        before = gpu.launches()
+        gpu.attn_prompt_dev(u.attn(q, out, lse, kv_heads=kv_heads),
+                            B.AttnKeys(k=k.data_ptr(), v=v.data_ptr(), rows=sum(nk),
+                                       cu_q=dq.data_ptr(), cu_k=dk.data_ptr(), seqs=len(nq),
+                                       causal=1), stream=u.stream())
+        torch.cuda.synchronize()
+        assert gpu.last_block_status() == 0
+        assert launches is None or gpu.launches() - before == launches
+        for i, c in enumerate(codes):
+            s = slice(cq[i], cq[i + 1])
+            _check_counts(out[s], lse[s], [nk[i] - nq[i] + 1 + j for j in range(nq[i])], c, dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("lengths", [[5000], [700, 2000, 31], [300] * 150])
+def test_decode_rising_keys(gpu, heads, kv_heads, dim, lengths):
+    """Every later tile of keys scores higher than all before, some by less than what a reference
+    has to move for and some by more: within a warp, between warps and between SMs."""
+    import torch
+    import attn_util as u
+    page = 16
+    held = [-(-m // page) for m in lengths]
+    cache = u.Cache(1, sum(held) + 1, kv_heads, page, dim, len(lengths),
+                    max(held) + 1).hold(lengths)
+    for s, m in enumerate(lengths):
+        t = torch.arange(m, device="cuda")
+        # (steps of 1, 2 and 4 times 2 = 8 * 0.25, and those are powers of e)
+        cache.k[0].transpose(1, 2)[cache.table[s][t // page].long(), t % page, :, 0] = \
+            (t // 16).bfloat16()[:, None]
+    q = torch.zeros(len(lengths), heads, dim, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = torch.tensor([8.0, 1.0, -8.0], device="cuda").bfloat16().repeat(heads)[:heads]
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    a = u.attn(q, out, lse, kv_heads=kv_heads, scale=0.25)
+    gpu.attn_decode_dev(a, cache.c, 0, None, stream=u.stream())
+    torch.cuda.synchronize()
+    assert cache.status() == 0
+    for s in range(min(3, len(lengths))):
+        k, v = cache.tokens(0, s)
+        u.check(out[s:s + 1], lse[s:s + 1],
+                u.exact(q[s:s + 1], k, v, u.ints([lengths[s]]), 0.25))
