@@ -94,7 +94,7 @@ extern "C" int apus_cuda_kv_extend_dev(const ApusCudaKvCache *kv, const int32_t 
     KvView v;
     if (kv_view(kv, "kv_extend_dev", &v)) return 1;
     if (!n && (!d_slot || !rows)) return 0;       /* (without a list no row has a place) */
-    if ((n && !d_cu) || n > kv->seqs || (d_slot && rows > 0x7fffffff))
+    if ((n && !d_cu) || n > kv->seqs || (d_slot && rows > (1u << 30)))
         return fail("kv_extend_dev: bad args");
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
@@ -109,7 +109,7 @@ extern "C" int apus_cuda_kv_free_dev(const ApusCudaKvCache *kv, const int32_t *d
     KvView v;
     if (kv_view(kv, "kv_free_dev", &v)) return 1;
     if (!n) return 0;
-    if (n > 0x7fffffff || (!d_seq && n > kv->seqs)) return fail("kv_free_dev: bad args");
+    if (n > (1u << 30) || (!d_seq && n > kv->seqs)) return fail("kv_free_dev: bad args");
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (ctx_init()) return 1;
     DeviceGuard dev(g_ctx->device);

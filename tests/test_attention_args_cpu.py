@@ -120,6 +120,15 @@ def test_a_table_too_large_to_count_is_refused(be, B):
         be.kv_free_dev(cache(B, seqs=1 << 10, max_pages=1 << 21), BIG, 1)
 
 
+def test_lists_whose_count_a_step_would_take_past_31_bits_are_refused(be, B):
+    c = cache(B)
+    for call in (lambda: be.kv_extend_dev(c, BIG, BIG, 1, BIG, (1 << 30) + 1),
+                 lambda: be.kv_extend_dev(c, None, None, 0, BIG, (1 << 31) - 1),
+                 lambda: be.kv_free_dev(c, BIG, (1 << 31) - 1)):
+        with pytest.raises(B.BackendError, match="bad args"):
+            call()
+
+
 def test_rope_and_cache_have_to_agree(be, B):
     for r, c, layer, slot in ((rope(B), cache(B, kv_heads=1), 0, BIG),
                               (rope(B), cache(B), 1, BIG), (rope(B), cache(B), 0, None),
