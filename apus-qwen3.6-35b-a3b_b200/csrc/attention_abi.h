@@ -407,14 +407,17 @@ extern "C" int apus_cuda_attn_prompt_dev(const ApusCudaAttn *a, const ApusCudaAt
     Ordered ord(c, st);
     if (ord.rc) return 1;
     /* Tiles that leave SMs idle share their keys, by four steps of 128 at least: the second kernel
-     * takes as long as two or three.  head_dim 256, 2 key heads: 16 rows over 4096 keys 52 -> 31
-     * us, 128 rows over 30128 331 -> 77, one row over 1000 20 -> 17.  Where the parts would fill
-     * the SMs, their way through memory takes longer than a few steps: 400 rows over 1000 keys 21
-     * -> 26, so only from sixteen steps on.
+     * takes as long as two or three.  head_dim 256, 2 key heads: 16 rows over 4096 keys 48 -> 28
+     * us, 128 rows over 30128 320 -> 68, one row over 1000 17 -> 16 (head_dim 64: 35 -> 15, 231 ->
+     * 39, 12 -> 11).  Where the parts would fill the SMs, their way through memory takes longer than a
+     * few steps: 400 rows over 1000 keys 21 -> 26, so only from sixteen steps on.  (Found at 256: at
+     * 64 such rows are 26 tiles, which do not fill them, and are shared, 12.5 -> 16.2.)
+     *
      * How many steps a tile has is on the device; the caller may say how many keys the longest
-     * sequence has.  Else all of them count, which one sequence may hold nearly alone: a row over 4000
-     * beside seven over 50 would take 49 us by the mean, and takes 19.  Where they are even, parts are short
-     * or empty without that number: eight rows over 200 keys each 14.3 us, 9.5 with it. */
+     * sequence has.  Else all of them count, which one sequence may hold nearly alone: a row over
+     * 4000 beside seven over 50 would take 48 us by the mean, and takes 18.  Where they are even,
+     * parts are short or empty without that number: eight rows over 200 keys each 13.1 us, 9.5 with
+     * it. */
     const size_t most = keys->longest && keys->longest < keys->rows ? keys->longest : keys->rows;
     const size_t steps = (most + AP_ROWS - 1) / AP_ROWS;
     size_t splits = (size_t)c->sm_count / p.items;

@@ -16,6 +16,11 @@
  * changes nothing.  What moves bytes (kv_apply_kernel) runs on all SMs and reads the plan: its
  * bound is HBM, each page read once and written once (241 MB moved together: 75 us, 6.4 TB/s of
  * reads and writes).
+ *
+ * One SM's loads bound a plan over a large pool: 0.08 to 0.09 us a thousand pages for each look at refs
+ * (two to find free pages, three to close up).  Closing up with nothing to move takes 5 us over
+ * 2000 pages, 34 over 100 000, 146 over 500 000; 8192 tokens of 256 sequences with their places 20
+ * us over 8192 pages, 37 and 102; tokens that need no page 7, and 8 with places, over any pool.
  */
 #pragma once
 #include <cuda_runtime.h>

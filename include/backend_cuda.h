@@ -554,11 +554,14 @@ int apus_cuda_bf16_gemv_dev(const uint16_t *d_w, const uint16_t *d_x, uint16_t *
  * Net-new beside the engine's CPU kernels (c/attn.h: one sequence, one plain cache): what a
  * server needs between the projections of a full-attention layer.  All pointers are device
  * pointers of the backend's device, BF16 tensors as codes; calls enqueue on `stream`, do not
- * synchronise, allocate nothing once the backend is enabled, and may be captured in a graph
+ * synchronise, allocate nothing once the backend is enabled (which sets 49 MB aside for unfinished
+ * sums), and may be captured in a graph
  * (attention sums up in the shared workspace: one stream order of graphs, as for the block).
  * Tensors are addressed by rows (2^30 at most, as of any list): `stride` elements from one row (token) to
  * the next (0: heads * head_dim), heads side by side within a row; addresses and strides in multiples
- * of 16 bytes.
+ * of 16 bytes.  A projection that gives each head its query and then its gate, 2 * head_dim apart,
+ * has no such stride: the rows of its weight are put in order once, all heads' queries before all
+ * gates (then both strides are 2 * heads * head_dim).
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 times as many: head h
  * reads key head h / (heads / kv_heads). */
 
